@@ -31,12 +31,16 @@ def sources():
     return sorted(glob.glob(os.path.join(_CSRC, "*.hip")))
 
 
+def _shared_deps():
+    """What every object depends on: the headers, and this file with its compiler flags."""
+    return glob.glob(os.path.join(_CSRC, "*.h")) + [os.path.abspath(__file__)]
+
+
 def _stale() -> bool:
     if not os.path.exists(LIB_PATH):
         return True
     t = os.path.getmtime(LIB_PATH)
-    deps = sources() + glob.glob(os.path.join(_CSRC, "*.h"))
-    return any(os.path.getmtime(d) > t for d in deps)
+    return any(os.path.getmtime(d) > t for d in sources() + _shared_deps())
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -47,13 +51,15 @@ def build(force: bool = False, verbose: bool = False) -> str:
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     objs = []
     procs = []
+    # no packed fp32 instructions: some forms that the compiler makes of ordinary float code have given wrong results
+    # now and then on this hardware, with no error (the host pass warns that it does not know the feature: harmless)
     flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-I", _CSRC,
-             "-Wno-unused-result"]
+             "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+    newest = max(os.path.getmtime(d) for d in _shared_deps())
     for src in sources():
         obj = os.path.join(_OUT_DIR, os.path.basename(src).replace(".hip", ".o"))
         objs.append(obj)
-        if force or not os.path.exists(obj) or os.path.getmtime(obj) < max(
-                [os.path.getmtime(src)] + [os.path.getmtime(h) for h in glob.glob(os.path.join(_CSRC, "*.h"))]):
+        if force or not os.path.exists(obj) or os.path.getmtime(obj) < max(os.path.getmtime(src), newest):
             cmd = [hipcc, *flags, "-c", src, "-o", obj]
             if verbose:
                 print(" ".join(cmd))

@@ -5,6 +5,9 @@
                int8/fp8 quantisation, top-k sparsification, fused CE, confusion matrix.
 ``norm_ops`` — GroupNorm (+ReLU) forward/backward, single-model and client-stacked.
 ``transformer_ops`` — LayerNorm / GELU / attention / client-batched MFMA GEMM.
+``window_ops`` — causal sliding-window attention with sinks and a bucketed relative position bias, and its form for one
+               new token over a ring cache.
+``scan_ops`` — gated linear recurrence over long sequences.
 ``nn_ops``   — client-batched (grouped) conv / BN / ReLU / pooling / linear kernels
                used by the virtual-client engine (MFMA implicit GEMM).
 """
@@ -45,6 +48,8 @@ from .fl_ops import (
     pack_conv_shadow,
 )
 from .norm_ops import FusedGroupNorm, fuse_group_norm, group_norm
+from .scan_ops import gated_scan
+from .window_ops import relative_bucket_starts, window_attention, window_attention_step, window_cache_fill
 
 
 def build(force: bool = False):

@@ -1,0 +1,410 @@
+// Gated linear recurrence (driven by ops/scan_ops.py), per sequence and feature:
+//   f_t = σ(gate_t),  h_t = f_t h_{t−1} + (1 − f_t) x_t,  y_t = h_t
+//   backward, with G_t = f_t δ_t handed on to step t − 1:  δ_t = dy_t + G_{t+1} (dh_T for the last step)
+//   dx_t = (1 − f_t) δ_t,  dgate_t = δ_t (h_{t−1} − x_t) f_t (1 − f_t),  dh_0 = G_1
+// A masked step has f = 1 and takes nothing: the state passes it, y, dx and dgate are zero there.
+//
+// Any run of steps is an affine map of the state, h → A h + B, and maps compose: a workgroup owns 32·V features of one
+// sequence and walks the time in tiles of 64 steps; 8 groups of 32 lanes take 8 steps each in registers, put their maps
+// into LDS, and every group composes those before it. The carried state stays in fp32 registers; x and gate are read
+// once. The forward leaves the state before every tile (fp32, 1/64 of the states): the backward recomputes the
+// others in registers from there, so it reads x, gate and dy only and loses nothing to the rounding of y.
+// Few features and a long time: the time is cut into segments, whose maps a first kernel forms (same reads); the
+// workgroups of the second compose those before (after, backward) their segment. Order fixed, no atomics.
+#include "common.h"
+
+namespace scan {
+
+constexpr int kTile = 64, kGroups = 8, kSteps = kTile / kGroups;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Args {
+  const void *x, *gate, *dy;
+  void *y, *dx, *dgate;
+  const float *h0, *dh;
+  float *hT, *dh0, *ckpt, *agg;
+  const uint8_t* mask;
+  int64_t xs[3], gs[3], dys[3], ys[3], ms[3];   // element strides over client, time and sequence; y, dx and dgate share ys
+  int C, T, B, H, nseg, tps;                    // tps: tiles of a segment
+};
+
+template <typename T, int V> struct Vec;
+template <> struct Vec<uint16_t, 2> {
+  typedef uint32_t raw;
+  static __device__ __forceinline__ void get(raw u, float* f) {
+    f[0] = __uint_as_float(u << 16);
+    f[1] = __uint_as_float(u & 0xffff0000u);
+  }
+  static __device__ __forceinline__ raw put(const float* f) {
+    return (uint32_t)f32_to_bf16(f[0]) | ((uint32_t)f32_to_bf16(f[1]) << 16);
+  }
+};
+template <> struct Vec<uint16_t, 1> {
+  typedef uint16_t raw;
+  static __device__ __forceinline__ void get(raw u, float* f) { f[0] = bf16_to_f32(u); }
+  static __device__ __forceinline__ raw put(const float* f) { return f32_to_bf16(f[0]); }
+};
+template <> struct Vec<float, 2> {
+  typedef float2 raw;
+  static __device__ __forceinline__ void get(raw u, float* f) {
+    f[0] = u.x;
+    f[1] = u.y;
+  }
+  static __device__ __forceinline__ raw put(const float* f) { return make_float2(f[0], f[1]); }
+};
+template <> struct Vec<float, 1> {
+  typedef float raw;
+  static __device__ __forceinline__ void get(raw u, float* f) { f[0] = u; }
+  static __device__ __forceinline__ raw put(const float* f) { return f[0]; }
+};
+
+// f = σ(g) and 1 − f = e^−g f, without the cancellation of the difference; below −80 f is smaller than any state's
+// last bit (and e^−g stays finite)
+__device__ __forceinline__ void gates(float g, float& f, float& keep) {
+  const float c = g < -80.f ? -80.f : g;
+  const float e = __builtin_amdgcn_exp2f(c * -kLog2e);
+  f = __builtin_amdgcn_rcpf(1.f + e);
+  keep = e * f;
+}
+
+// where a workgroup and a thread stand
+template <int V> struct At {
+  int c, b, seg, lane, grp, j;
+  bool on;
+  __device__ __forceinline__ explicit At(const Args& a) {
+    const int nft = (a.H + 32 * V - 1) / (32 * V);
+    int64_t id = blockIdx.x;
+    const int ft = (int)(id % nft);
+    id /= nft;
+    seg = (int)(id % a.nseg);
+    id /= a.nseg;
+    b = (int)(id % a.B);
+    c = (int)(id / a.B);
+    lane = threadIdx.x & 31;
+    grp = threadIdx.x >> 5;
+    j = (ft * 32 + lane) * V;
+    on = j < a.H;
+  }
+};
+
+// one stream of a thread's 8 steps of a tile
+template <typename T, int V> struct Steps {
+  typename Vec<T, V>::raw r[kSteps];
+  __device__ __forceinline__ void load(const T* p, int64_t st, int t0, int T_, bool on) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      r[i] = typename Vec<T, V>::raw{};
+      if (on && t0 + i < T_) r[i] = *reinterpret_cast<const typename Vec<T, V>::raw*>(p + (t0 + i) * st);
+    }
+  }
+};
+
+// bit i: step t0 + i exists and is no padding
+__device__ __forceinline__ uint32_t real_steps(const uint8_t* m, int64_t st, int t0, int T_) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i)
+    if (t0 + i < T_ && (!m || m[(t0 + i) * st])) bits |= 1u << i;
+  return bits;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void step_values(const Steps<T, V>& x, const Steps<T, V>& g, uint32_t bits, int i, float* f,
+                                            float* keep, float* xv) {
+  float gv[V];
+  Vec<T, V>::get(g.r[i], gv);
+  Vec<T, V>::get(x.r[i], xv);
+  const bool real = (bits >> i) & 1;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    gates(gv[v], f[v], keep[v]);
+    f[v] = real ? f[v] : 1.f;
+    keep[v] = real ? keep[v] : 0.f;
+    xv[v] = real ? xv[v] : 0.f;
+  }
+}
+
+template <typename T, int V> __global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
+  __shared__ float sA[2][kGroups][32 * V], sB[2][kGroups][32 * V];
+  const At<V> at(a);
+  const int ntile = (a.T + kTile - 1) / kTile;
+  const int k0 = at.seg * a.tps, k1 = k0 + a.tps < ntile ? k0 + a.tps : ntile;
+  const T* x = (const T*)a.x + at.c * a.xs[0] + at.b * a.xs[2] + at.j;
+  const T* g = (const T*)a.gate + at.c * a.gs[0] + at.b * a.gs[2] + at.j;
+  T* y = (T*)a.y + at.c * a.ys[0] + at.b * a.ys[2] + at.j;
+  const uint8_t* m = a.mask ? a.mask + at.c * a.ms[0] + at.b * a.ms[2] : nullptr;
+  const int64_t chan = ((int64_t)at.c * a.B + at.b) * a.H + at.j;
+  float h[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = at.on && a.h0 ? a.h0[chan + v] : 0.f;
+  for (int s = 0; s < at.seg && at.on; ++s) {      // the segments before this one
+    const float* p = a.agg + (((int64_t)at.c * a.B + at.b) * a.nseg + s) * 2 * a.H + at.j;
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = fmaf(p[v], h[v], p[a.H + v]);
+  }
+  Steps<T, V> rx, rg;
+  uint32_t bits = real_steps(m, a.ms[1], k0 * kTile + at.grp * kSteps, a.T);
+  rx.load(x, a.xs[1], k0 * kTile + at.grp * kSteps, a.T, at.on);
+  rg.load(g, a.gs[1], k0 * kTile + at.grp * kSteps, a.T, at.on);
+  for (int k = k0; k < k1; ++k) {
+    const int t0 = k * kTile + at.grp * kSteps, buf = k & 1;
+    float f[kSteps][V], in[kSteps][V], A[V], Bv[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      A[v] = 1.f;
+      Bv[v] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      float keep[V], xv[V];
+      step_values<T, V>(rx, rg, bits, i, f[i], keep, xv);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        in[i][v] = keep[v] * xv[v];
+        A[v] *= f[i][v];
+        Bv[v] = fmaf(f[i][v], Bv[v], in[i][v]);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      sA[buf][at.grp][at.lane * V + v] = A[v];
+      sB[buf][at.grp][at.lane * V + v] = Bv[v];
+    }
+    const uint32_t now = bits;
+    if (k + 1 < k1) {
+      bits = real_steps(m, a.ms[1], t0 + kTile, a.T);
+      rx.load(x, a.xs[1], t0 + kTile, a.T, at.on);
+      rg.load(g, a.gs[1], t0 + kTile, a.T, at.on);
+    }
+    if (a.ckpt && at.grp == 0 && at.on) {
+      float* p = a.ckpt + (((int64_t)at.c * ntile + k) * a.B + at.b) * a.H + at.j;
+#pragma unroll
+      for (int v = 0; v < V; ++v) p[v] = h[v];
+    }
+    __syncthreads();
+    float s[V];
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (i == at.grp) s[v] = h[v];
+        h[v] = fmaf(sA[buf][i][at.lane * V + v], h[v], sB[buf][i][at.lane * V + v]);
+      }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      float o[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        s[v] = fmaf(f[i][v], s[v], in[i][v]);
+        o[v] = (now >> i) & 1 ? s[v] : 0.f;
+      }
+      if (at.on && t0 + i < a.T)
+        *reinterpret_cast<typename Vec<T, V>::raw*>(y + (t0 + i) * a.ys[1]) = Vec<T, V>::put(o);
+    }
+  }
+  if (at.on && at.grp == 0 && k1 == ntile)
+#pragma unroll
+    for (int v = 0; v < V; ++v) a.hT[chan + v] = h[v];
+}
+
+template <typename T, int V> __global__ __launch_bounds__(256) void bwd_kernel(const Args a) {
+  __shared__ float sA[2][kGroups][32 * V], sB[2][kGroups][32 * V], sG[2][kGroups][32 * V];
+  const At<V> at(a);
+  const int ntile = (a.T + kTile - 1) / kTile;
+  const int k0 = at.seg * a.tps, k1 = k0 + a.tps < ntile ? k0 + a.tps : ntile;
+  const T* x = (const T*)a.x + at.c * a.xs[0] + at.b * a.xs[2] + at.j;
+  const T* g = (const T*)a.gate + at.c * a.gs[0] + at.b * a.gs[2] + at.j;
+  const T* dy = (const T*)a.dy + at.c * a.dys[0] + at.b * a.dys[2] + at.j;
+  T* dx = (T*)a.dx + at.c * a.ys[0] + at.b * a.ys[2] + at.j;
+  T* dg = (T*)a.dgate + at.c * a.ys[0] + at.b * a.ys[2] + at.j;
+  const uint8_t* m = a.mask ? a.mask + at.c * a.ms[0] + at.b * a.ms[2] : nullptr;
+  const int64_t chan = ((int64_t)at.c * a.B + at.b) * a.H + at.j;
+  float G[V], h[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) G[v] = at.on && a.dh ? a.dh[chan + v] : 0.f;
+  for (int s = a.nseg - 1; s > at.seg && at.on; --s) {      // the segments after this one
+    const float* p = a.agg + (((int64_t)at.c * a.B + at.b) * a.nseg + s) * 2 * a.H + at.j;
+#pragma unroll
+    for (int v = 0; v < V; ++v) G[v] = fmaf(p[v], G[v], p[a.H + v]);
+  }
+  Steps<T, V> rx, rg, rd;
+  float hn[V];                                               // the state before the tile
+  uint32_t bits;
+  auto load = [&](int k) {
+    const int t0 = k * kTile + at.grp * kSteps;
+    bits = real_steps(m, a.ms[1], t0, a.T);
+    rx.load(x, a.xs[1], t0, a.T, at.on);
+    rg.load(g, a.gs[1], t0, a.T, at.on);
+    rd.load(dy, a.dys[1], t0, a.T, at.on);
+    const float* p = a.ckpt + (((int64_t)at.c * ntile + k) * a.B + at.b) * a.H + at.j;
+#pragma unroll
+    for (int v = 0; v < V; ++v) hn[v] = at.on ? p[v] : 0.f;
+  };
+  load(k1 - 1);
+  for (int k = k1 - 1; k >= k0; --k) {
+    const int t0 = k * kTile + at.grp * kSteps, buf = k & 1;
+    float f[kSteps][V], keep[kSteps][V], xv[kSteps][V], d[kSteps][V], A[V], Bv[V], Gv[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      A[v] = 1.f;
+      Bv[v] = Gv[v] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      step_values<T, V>(rx, rg, bits, i, f[i], keep[i], xv[i]);
+      Vec<T, V>::get(rd.r[i], d[i]);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        d[i][v] = (bits >> i) & 1 ? d[i][v] : 0.f;
+        A[v] *= f[i][v];
+        Bv[v] = fmaf(f[i][v], Bv[v], keep[i][v] * xv[i][v]);
+      }
+    }
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; --i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) Gv[v] = f[i][v] * (d[i][v] + Gv[v]);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      sA[buf][at.grp][at.lane * V + v] = A[v];
+      sB[buf][at.grp][at.lane * V + v] = Bv[v];
+      sG[buf][at.grp][at.lane * V + v] = Gv[v];
+      h[v] = hn[v];
+    }
+    if (k > k0) load(k - 1);
+    __syncthreads();
+    float s[V], e[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float tA[kGroups];
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        tA[i] = sA[buf][i][at.lane * V + v];
+        if (i == at.grp) s[v] = h[v];
+        h[v] = fmaf(tA[i], h[v], sB[buf][i][at.lane * V + v]);
+      }
+#pragma unroll
+      for (int i = kGroups - 1; i >= 0; --i) {
+        if (i == at.grp) e[v] = G[v];
+        G[v] = fmaf(tA[i], G[v], sG[buf][i][at.lane * V + v]);
+      }
+    }
+    // dgate without δ: (h_{t−1} − x_t) f_t (1 − f_t), formed on the way forward
+    float q[kSteps][V];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        q[i][v] = (s[v] - xv[i][v]) * (f[i][v] * keep[i][v]);
+        s[v] = fmaf(f[i][v], s[v], keep[i][v] * xv[i][v]);
+      }
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; --i) {
+      float ox[V], og[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float dl = d[i][v] + e[v];
+        ox[v] = keep[i][v] * dl;
+        og[v] = q[i][v] * dl;
+        e[v] = f[i][v] * dl;
+      }
+      if (at.on && t0 + i < a.T) {
+        *reinterpret_cast<typename Vec<T, V>::raw*>(dx + (t0 + i) * a.ys[1]) = Vec<T, V>::put(ox);
+        *reinterpret_cast<typename Vec<T, V>::raw*>(dg + (t0 + i) * a.ys[1]) = Vec<T, V>::put(og);
+      }
+    }
+  }
+  if (at.on && at.grp == 0 && k0 == 0 && a.dh0)
+#pragma unroll
+    for (int v = 0; v < V; ++v) a.dh0[chan + v] = G[v];
+}
+
+// the map of every segment: forward h → A h + B (from x), backward G → A G + B (from dy)
+template <typename T, int V, bool BWD> __global__ __launch_bounds__(256) void agg_kernel(const Args a) {
+  __shared__ float sA[kGroups][32 * V], sB[kGroups][32 * V];
+  const At<V> at(a);
+  const int ntile = (a.T + kTile - 1) / kTile;
+  const int k0 = at.seg * a.tps, k1 = k0 + a.tps < ntile ? k0 + a.tps : ntile;
+  const T* g = (const T*)a.gate + at.c * a.gs[0] + at.b * a.gs[2] + at.j;
+  const T* o = BWD ? (const T*)a.dy + at.c * a.dys[0] + at.b * a.dys[2] + at.j
+                   : (const T*)a.x + at.c * a.xs[0] + at.b * a.xs[2] + at.j;
+  const int64_t ot = BWD ? a.dys[1] : a.xs[1];
+  const uint8_t* m = a.mask ? a.mask + at.c * a.ms[0] + at.b * a.ms[2] : nullptr;
+  // a group walks a run of the segment of its own: its map is formed without a barrier
+  const int run = ((k1 - k0) * kTile + kGroups - 1) / kGroups;       // a multiple of 8: a tile is 8 groups of 8 steps
+  const int ta = k0 * kTile + at.grp * run, tb = ta + run;
+  float A[V], Bv[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    A[v] = 1.f;
+    Bv[v] = 0.f;
+  }
+  Steps<T, V> rg, ro;
+  uint32_t bits;
+  const int n = run / kSteps;
+  auto load = [&](int i) {
+    const int t0 = BWD ? tb - (i + 1) * kSteps : ta + i * kSteps;
+    bits = real_steps(m, a.ms[1], t0, a.T);
+    rg.load(g, a.gs[1], t0, a.T, at.on);
+    ro.load(o, ot, t0, a.T, at.on);
+  };
+  load(0);
+  for (int i = 0; i < n; ++i) {
+    const Steps<T, V> cg = rg, co = ro;
+    const uint32_t now = bits;
+    if (i + 1 < n) load(i + 1);
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u) {
+      const int r = BWD ? kSteps - 1 - u : u;
+      float f[V], keep[V], ov[V];
+      step_values<T, V>(co, cg, now, r, f, keep, ov);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        A[v] *= f[v];
+        Bv[v] = BWD ? f[v] * (ov[v] + Bv[v]) : fmaf(f[v], Bv[v], keep[v] * ov[v]);
+      }
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    sA[at.grp][at.lane * V + v] = A[v];
+    sB[at.grp][at.lane * V + v] = Bv[v];
+  }
+  __syncthreads();
+  if (at.grp || !at.on) return;
+  float* p = a.agg + (((int64_t)at.c * a.B + at.b) * a.nseg + at.seg) * 2 * a.H + at.j;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float A1 = 1.f, B1 = 0.f;
+#pragma unroll
+    for (int u = 0; u < kGroups; ++u) {
+      const int i = BWD ? kGroups - 1 - u : u;
+      B1 = fmaf(sA[i][at.lane * V + v], B1, sB[i][at.lane * V + v]);
+      A1 *= sA[i][at.lane * V + v];
+    }
+    p[v] = A1;
+    p[a.H + v] = B1;
+  }
+}
+
+template <typename T, int V> int launch(const Args& a, bool bwd, hipStream_t st) {
+  const int64_t n = (int64_t)a.C * a.B * a.nseg * ((a.H + 32 * V - 1) / (32 * V));
+  const dim3 grid((unsigned)n), block(256);
+  if (a.nseg > 1) {
+    if (bwd) hipLaunchKernelGGL((agg_kernel<T, V, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((agg_kernel<T, V, false>), grid, block, 0, st, a);
+    const int rc = (int)hipGetLastError();
+    if (rc) return rc;
+  }
+  if (bwd) hipLaunchKernelGGL((bwd_kernel<T, V>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((fwd_kernel<T, V>), grid, block, 0, st, a);
+  return (int)hipGetLastError();
+}
+
+}  // namespace scan
+
+// vec: 2 where every row starts at a multiple of two elements and H is even, else 1
+FA_EXPORT int fa_gated_scan(const scan::Args* a, int bf16, int vec, int bwd, hipStream_t stream) {
+  if (bf16) return vec == 2 ? scan::launch<uint16_t, 2>(*a, bwd, stream) : scan::launch<uint16_t, 1>(*a, bwd, stream);
+  return vec == 2 ? scan::launch<float, 2>(*a, bwd, stream) : scan::launch<float, 1>(*a, bwd, stream);
+}

@@ -1,0 +1,1012 @@
+// Causal sliding-window attention with sinks and a bucketed relative position bias, for long text (driven by
+// ops/window_ops.py): forward, backward, and the form for one new token over a ring cache.
+//
+//   visible(i, j) = j <= i and (i - j < W or j < sinks), tokens i and j both real (mask)
+//   s_ij = scale q_i·k_j + bias[c, h, bucket(i − j)],  p = softmax over the visible j,  o_i = Σ p_ij v_j
+//   D_i = dO_i·o_i,  dS = p (dO_i·v_j − D_i),  dq_i = scale Σ dS k_j,  dk_j = scale Σ dS q_i,  dv_j = Σ p dO_i
+//   dbias[c, h, b] = Σ over the client's sequences and the visible pairs of bucket b of dS
+//
+// Layouts: token-major rows [sequence · S + token][heads · D], head h at column D·h; H query heads share KV heads of
+// keys and values (head h reads kv head h / (H / KV)). Storage bf16 or fp32, sums and statistics fp32.
+//
+// All kernels work on 32×32 blocks of scores with the same maps of lanes (l = lane, hh = l >> 5):
+//   C / D of the 32×32 products: column l & 31, row κ(r) + 4·hh, κ(r) = (r & 3) + 8·(r >> 2), r = 0 … 15;
+//   row operands (both sides of a product over the head dim): lane l holds 16 bytes of row l & 31, unit 2c + hh of
+//   the row for chunk c — one 32×32×16 bf16 product, or four 32×32×2 fp32 products; the order of the dims inside a
+//   chunk is the same on both sides, so the sum is over all of them;
+//   column operands (products over 32 rows of an LDS tile): the 16 accumulators of a lane ARE the other operand,
+//   with the rows taken in the order κ(r) + 4·hh, so probabilities never leave the registers.
+#include "common.h"
+#include <type_traits>
+
+namespace win {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short v4i16 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxBuckets = 128;
+constexpr int kLutOff = 62;      // a processed 32×32 block holds distances >= −62 (the negative ones are masked)
+constexpr int kBinPad = 64;      // distances of a block that starts below max_distance end below max_distance + 62
+
+struct Args {
+  const void *q, *k, *v, *dout;
+  void *o, *olo, *dq, *dk, *dv;
+  float *lse, *dsum, *part, *bpart, *dbias;
+  const uint8_t* mask;
+  const float* bias;
+  int64_t ldq, ldk, ldv, lddo;
+  int N, S, H, KV, C, W, sinks, NB, maxd;
+  int nchunk, qchunk;            // sink pass of the backward: chunks of queries
+  float scale;
+  int start[kMaxBuckets];        // first distance of every bucket
+};
+
+__device__ __forceinline__ int kappa(int r) { return (r & 3) + 8 * (r >> 2); }
+
+// consecutive work items to the same XCD (workgroup ids go round the 8 of them), so that tiles which read the same
+// keys meet in one L2
+__device__ __forceinline__ int xcd_swizzle(int id, int n) {
+  const int per = n >> 3;
+  return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
+}
+
+template <typename T> struct Elem;
+template <> struct Elem<uint16_t> {
+  static constexpr int kPad = 8;
+  static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  }
+  static __device__ __forceinline__ float dot(uint4 a, uint4 b, float s) {
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), s);
+      s = fmaf(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), s);
+    }
+    return s;
+  }
+  // four consecutive columns; lo (optional): what the rounding left over
+  static __device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, float d) {
+    uint2 u;
+    u.x = (uint32_t)f32_to_bf16(a) | ((uint32_t)f32_to_bf16(b) << 16);
+    u.y = (uint32_t)f32_to_bf16(c) | ((uint32_t)f32_to_bf16(d) << 16);
+    *reinterpret_cast<uint2*>(p) = u;
+  }
+  static __device__ __forceinline__ float left(float a) { return a - bf16_to_f32(f32_to_bf16(a)); }
+};
+template <> struct Elem<float> {
+  static constexpr int kPad = 4;
+  static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
+    const float4 x = __builtin_bit_cast(float4, a), y = __builtin_bit_cast(float4, b);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, y.x, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, y.y, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, y.z, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, y.w, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float dot(uint4 a, uint4 b, float s) {
+    const float4 x = __builtin_bit_cast(float4, a), y = __builtin_bit_cast(float4, b);
+    return fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s))));
+  }
+  static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
+    *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+  }
+  static __device__ __forceinline__ float left(float) { return 0.f; }
+};
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
+}
+
+// A head's rows and how they lie in registers and LDS
+template <typename T, int D> struct Row {
+  static constexpr int U = D * (int)sizeof(T) / 16;   // 16-byte units of a row
+  static constexpr int NC = U / 2;                    // chunks: a unit for either half of the wave
+  static constexpr int E = 16 / (int)sizeof(T);       // elements of a unit
+  static constexpr int P = D + Elem<T>::kPad;         // LDS pitch: 16 rows' units lie on different banks
+  static constexpr int DB = D / 32;                   // 32-column blocks
+
+  static __device__ __forceinline__ uint4 unit(const T* row, int u) {
+    return *reinterpret_cast<const uint4*>(row + u * E);
+  }
+  // this lane's fragments of row l & 31 (zero where the row is none)
+  static __device__ __forceinline__ void frags(uint4* f, const T* row, bool real, int hh) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) f[c] = real ? unit(row, 2 * c + hh) : make_uint4(0, 0, 0, 0);
+  }
+  // 32 rows of an LDS tile × this lane's column: Σ over the head dim
+  static __device__ __forceinline__ f32x16 rows(const T* tile, const uint4* f, int lane) {
+    f32x16 acc = zero16();
+    const T* row = tile + (lane & 31) * P;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc = Elem<T>::mma(unit(row, 2 * c + (lane >> 5)), f[c], acc);
+    return acc;
+  }
+  // acc[db][column][row] += Σ over 32 rows of the LDS tile of tile[row][32 db + ·] · p[row]
+  static __device__ __forceinline__ void cols(f32x16* acc, const T* tile, const float* p, int lane) {
+    if constexpr (sizeof(T) == 2) {
+      bf16x8 b[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[t][j] = (__bf16)p[8 * t + j];
+      const int g = lane >> 4, i = lane & 15;
+      // 16 lanes read 4 rows × 16 columns and get a column of 4 rows each
+      const uint16_t* at = reinterpret_cast<const uint16_t*>(tile) + (4 * (g >> 1) + (i >> 2)) * P + 16 * (g & 1) +
+                           4 * (i & 3);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const v4i16 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(at + 16 * t * P + 32 * db));
+          const v4i16 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(at + (16 * t + 8) * P + 32 * db));
+          union {
+            v4i16 h[2];
+            bf16x8 v;
+          } a;
+          a.h[0] = x;
+          a.h[1] = y;
+          acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b[t], acc[db], 0, 0, 0);
+        }
+    } else {
+      const float* at = reinterpret_cast<const float*>(tile) + 4 * (lane >> 5) * P + (lane & 31);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[kappa(r) * P + 32 * db], p[r], acc[db], 0, 0, 0);
+    }
+  }
+};
+
+// ROWS rows of a [·][D] source between registers and an LDS tile, NT threads; rows that are no tokens become zero, so
+// that what they hold (NaN included) reaches no product
+template <typename T, int D, int ROWS, int NT> struct Stage {
+  using R = Row<T, D>;
+  static constexpr int NI = ROWS * R::U / NT;
+  static_assert(NI >= 1 && ROWS * R::U % NT == 0, "staging");
+  uint4 reg[NI];
+  __device__ __forceinline__ void load(const T* src, int64_t ld, int row0, int end, const uint8_t* mask, int tid) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int u = tid + i * NT, row = row0 + u / R::U;
+      reg[i] = make_uint4(0, 0, 0, 0);
+      if (row < end && (!mask || mask[row])) reg[i] = R::unit(src + row * ld, u % R::U);
+    }
+  }
+  __device__ __forceinline__ void store(T* tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int u = tid + i * NT;
+      *reinterpret_cast<uint4*>(tile + (u / R::U) * R::P + (u % R::U) * R::E) = reg[i];
+    }
+  }
+};
+
+// lut[d + kLutOff] = bias of distance d in units of log 2, for −62 <= d < max_distance + 62
+__device__ __forceinline__ int lut_size(int maxd) { return maxd + 2 * kLutOff; }
+__device__ __forceinline__ void fill_lut(float* lut, const Args& a, int client, int h, int tid, int nt) {
+  const float* tab = a.bias + ((int64_t)client * a.H + h) * a.NB;
+  for (int t = tid; t < lut_size(a.maxd); t += nt) {
+    int b = 0;
+    for (int i = 1; i < a.NB; ++i) b += (t - kLutOff >= a.start[i]) ? 1 : 0;
+    lut[t] = tab[b] * kLog2e;
+  }
+}
+
+// the key tiles that a tile of queries [q0, q0 + nq) sees: `first` tiles of sinks, then lo … hi
+struct KeyTiles {
+  int first, lo, count;
+  __device__ __forceinline__ KeyTiles(const Args& a, int q0, int nq, int bk) {
+    lo = q0 - a.W + 1 > 0 ? (q0 - a.W + 1) / bk : 0;
+    const int last = q0 + nq - 1 < a.S - 1 ? q0 + nq - 1 : a.S - 1;
+    first = (a.sinks + bk - 1) / bk;
+    if (first > lo) first = lo;
+    count = first + last / bk - lo + 1;
+  }
+  __device__ __forceinline__ int at(int i) const { return i < first ? i : lo + i - first; }
+};
+
+// ----------------------------------------------------------------------------------------------------------------
+// Forward: a wave owns 32 queries (its columns), the workgroup 32·NW of one head, and walks the visible keys in tiles
+// of BK with a running maximum and sum. The next tile's rows are in flight in registers during a tile's products.
+// Probabilities are rounded to the storage type for the product with v (half a step each, 2^-8 in bf16, and the sum is
+// of the unrounded ones). EXACT (bf16, before a gradient of the bias): what that rounding leaves over goes through a
+// second product and what the output's leaves over is kept, so that D = dO·o is good to 2^-16 — dbias is fp32.
+// ----------------------------------------------------------------------------------------------------------------
+template <typename T, int D, int NW, int BK, bool EXACT>
+__global__ __launch_bounds__(64 * NW) void fwd_kernel(const Args a) {
+  using R = Row<T, D>;
+  __shared__ __attribute__((aligned(16))) T Ks[BK * R::P];
+  __shared__ __attribute__((aligned(16))) T Vs[BK * R::P];
+  extern __shared__ float lut[];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
+  const int G = a.H / a.KV, nqt = (a.S + 32 * NW - 1) / (32 * NW);
+  int id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int g = id % G;
+  id /= G;
+  const int qt = id % nqt;
+  id /= nqt;
+  const int kv = id % a.KV, n = id / a.KV, h = kv * G + g;
+  const int64_t tok0 = (int64_t)n * a.S;
+  const T* kp = (const T*)a.k + tok0 * a.ldk + kv * D;
+  const T* vp = (const T*)a.v + tok0 * a.ldv + kv * D;
+  const uint8_t* mask = a.mask ? a.mask + tok0 : nullptr;
+  const int q0 = qt * 32 * NW, qw = q0 + 32 * w, qi = qw + (lane & 31);
+  const bool real = qi < a.S && (!mask || mask[qi]);
+  uint4 qf[R::NC];
+  R::frags(qf, (const T*)a.q + (tok0 + qi) * a.ldq + h * D, real, hh);
+  if (a.bias) fill_lut(lut, a, n / (a.N / a.C), h, tid, 64 * NW);
+  const KeyTiles tiles(a, q0, 32 * NW, BK);
+  const int count = __syncthreads_or(real) ? tiles.count : 0;
+  const float c2 = a.scale * kLog2e;
+  float m = -INFINITY, l = 0.f;
+  f32x16 acc[R::DB];
+#pragma unroll
+  for (int db = 0; db < R::DB; ++db) acc[db] = zero16();
+  Stage<T, D, BK, 64 * NW> sk, sv;
+  if (count) {
+    sk.load(kp, a.ldk, tiles.at(0) * BK, a.S, mask, tid);
+    sv.load(vp, a.ldv, tiles.at(0) * BK, a.S, mask, tid);
+  }
+  for (int it = 0; it < count; ++it) {
+    const int k0 = tiles.at(it) * BK;
+    __syncthreads();
+    sk.store(Ks, tid);
+    sv.store(Vs, tid);
+    __syncthreads();
+    if (it + 1 < count) {
+      sk.load(kp, a.ldk, tiles.at(it + 1) * BK, a.S, mask, tid);
+      sv.load(vp, a.ldv, tiles.at(it + 1) * BK, a.S, mask, tid);
+    }
+#pragma unroll
+    for (int sub = 0; sub < BK / 32; ++sub) {
+      const int kb = k0 + 32 * sub;
+      if (qw >= a.S || kb >= a.S || kb > qw + 31 || !(qw - kb - 31 < a.W || kb < a.sinks)) continue;
+      f32x16 s = R::rows(Ks + 32 * sub * R::P, qf, lane);
+      const uint32_t bits =
+          (uint32_t)__ballot(kb + (lane & 31) < a.S && (!mask || mask[kb + (lane & 31)])) >> (4 * hh);
+      const bool all = !__any(bits != (hh ? 0x0fffffffu : 0xffffffffu)) && kb + 31 <= qw &&
+                       (qw + 31 - kb < a.W || kb + 31 < a.sinks);
+      if (a.bias) {
+        if (qw - kb - 31 < a.maxd) {
+          const float* at = lut + kLutOff + qi - kb - 4 * hh;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, at[-kappa(r)]);
+        } else {
+          const float far = lut[lut_size(a.maxd) - 1];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, far);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= c2;
+      }
+      if (!all) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = kb + kappa(r) + 4 * hh;
+          const bool see = key <= qi && (qi - key < a.W || key < a.sinks) && ((bits >> kappa(r)) & 1);
+          s[r] = see ? s[r] : -INFINITY;
+        }
+      }
+      float mt = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
+      mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+      const float mn = fmaxf(m, mt), mu = mn == -INFINITY ? 0.f : mn;
+      if (__any(mn > m)) {
+        const float al = __builtin_amdgcn_exp2f(m - mu);
+        l *= al;
+#pragma unroll
+        for (int db = 0; db < R::DB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[db][r] *= al;
+      }
+      m = mn;
+      float p[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        p[r] = __builtin_amdgcn_exp2f(s[r] - mu);
+        l += p[r];
+      }
+      R::cols(acc, Vs + 32 * sub * R::P, p, lane);
+      if (EXACT) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] = Elem<T>::left(p[r]);
+        R::cols(acc, Vs + 32 * sub * R::P, p, lane);
+      }
+    }
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (qi >= a.S) return;
+  const float inv = real && l > 0.f ? 1.f / l : 0.f;
+  const int64_t at = (tok0 + qi) * (int64_t)(a.H * D) + h * D + 4 * hh;
+  const bool nan = real && !(l >= 0.f);   // a row of non-finite scores is what the formula makes of it
+#pragma unroll
+  for (int db = 0; db < R::DB; ++db)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = nan ? l : real ? acc[db][4 * c + j] * inv : 0.f;
+      Elem<T>::store4((T*)a.o + at + 32 * db + 8 * c, x[0], x[1], x[2], x[3]);
+      if (EXACT)
+        Elem<T>::store4((T*)a.olo + at + 32 * db + 8 * c, Elem<T>::left(x[0]), Elem<T>::left(x[1]),
+                        Elem<T>::left(x[2]), Elem<T>::left(x[3]));
+    }
+  if (a.lse && hh == 0)
+    a.lse[((int64_t)n * a.H + h) * a.S + qi] = nan ? l : real && l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+}
+
+// ----------------------------------------------------------------------------------------------------------------
+// Backward, dq (and D, dbias): the forward's walk. D_i = dO_i·o_i is formed from the forward's rounded output and
+// what its rounding left over, where dbias (fp32) needs it exact.
+// dbias: dS is summed per distance, in one order whatever the launch: a 32×32 block goes to LDS skewed by its row, so
+// that a column holds one distance, and a lane adds up a column and adds it to the wave's own bin of that distance;
+// blocks whose distances all lie in the last bucket are summed in registers.
+// ----------------------------------------------------------------------------------------------------------------
+template <typename T, int D, int NW, int BK, bool BIAS>
+__global__ __launch_bounds__(64 * NW) void dq_kernel(const Args a) {
+  using R = Row<T, D>;
+  __shared__ __attribute__((aligned(16))) T Ks[BK * R::P];
+  __shared__ __attribute__((aligned(16))) T Vs[BK * R::P];
+  __shared__ float skew[BIAS ? NW * 2048 : 1];
+  __shared__ float fars[NW];
+  extern __shared__ float lut[];                 // BIAS: lut, then NW × (maxd + kBinPad) bins
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
+  const int G = a.H / a.KV, nqt = (a.S + 32 * NW - 1) / (32 * NW);
+  int id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int g = id % G;
+  id /= G;
+  const int qt = id % nqt;
+  id /= nqt;
+  const int kv = id % a.KV, n = id / a.KV, h = kv * G + g;
+  const int64_t tok0 = (int64_t)n * a.S;
+  const T* kp = (const T*)a.k + tok0 * a.ldk + kv * D;
+  const T* vp = (const T*)a.v + tok0 * a.ldv + kv * D;
+  const uint8_t* mask = a.mask ? a.mask + tok0 : nullptr;
+  const int q0 = qt * 32 * NW, qw = q0 + 32 * w, qi = qw + (lane & 31);
+  const bool real = qi < a.S && (!mask || mask[qi]);
+  const int nbin = a.maxd + kBinPad;
+  float* bins = lut + lut_size(a.maxd) + w * nbin;
+  float* sk_w = skew + (BIAS ? w * 2048 : 0);
+  uint4 qf[R::NC], df[R::NC];
+  R::frags(qf, (const T*)a.q + (tok0 + qi) * a.ldq + h * D, real, hh);
+  R::frags(df, (const T*)a.dout + (tok0 + qi) * a.lddo + h * D, real, hh);
+  float Dq = 0.f, L = INFINITY;
+  if (real) {
+    const T* op = (const T*)a.o + (tok0 + qi) * (int64_t)(a.H * D) + h * D;
+    const T* lp = a.olo ? (const T*)a.olo + (tok0 + qi) * (int64_t)(a.H * D) + h * D : nullptr;
+#pragma unroll
+    for (int c = 0; c < R::NC; ++c) {
+      Dq = Elem<T>::dot(df[c], R::unit(op, 2 * c + hh), Dq);
+      if (sizeof(T) == 2 && lp) Dq = Elem<T>::dot(df[c], R::unit(lp, 2 * c + hh), Dq);
+    }
+    L = a.lse[((int64_t)n * a.H + h) * a.S + qi];
+  }
+  Dq += __shfl_xor(Dq, 32, 64);
+  if (qi < a.S && hh == 0) a.dsum[((int64_t)n * a.H + h) * a.S + qi] = Dq;
+  if (BIAS) {
+    fill_lut(lut, a, n / (a.N / a.C), h, tid, 64 * NW);
+    for (int i = lane; i < nbin; i += 64) bins[i] = 0.f;
+    for (int i = lane; i < 2048; i += 64) sk_w[i] = 0.f;
+  }
+  float far = 0.f;
+  const KeyTiles tiles(a, q0, 32 * NW, BK);
+  const int count = __syncthreads_or(real) ? tiles.count : 0;
+  const float c2 = a.scale * kLog2e;
+  f32x16 acc[R::DB];
+#pragma unroll
+  for (int db = 0; db < R::DB; ++db) acc[db] = zero16();
+  Stage<T, D, BK, 64 * NW> sk, sv;
+  if (count) {
+    sk.load(kp, a.ldk, tiles.at(0) * BK, a.S, mask, tid);
+    sv.load(vp, a.ldv, tiles.at(0) * BK, a.S, mask, tid);
+  }
+  for (int it = 0; it < count; ++it) {
+    const int k0 = tiles.at(it) * BK;
+    __syncthreads();
+    sk.store(Ks, tid);
+    sv.store(Vs, tid);
+    __syncthreads();
+    if (it + 1 < count) {
+      sk.load(kp, a.ldk, tiles.at(it + 1) * BK, a.S, mask, tid);
+      sv.load(vp, a.ldv, tiles.at(it + 1) * BK, a.S, mask, tid);
+    }
+#pragma unroll
+    for (int sub = 0; sub < BK / 32; ++sub) {
+      const int kb = k0 + 32 * sub;
+      if (qw >= a.S || kb >= a.S || kb > qw + 31 || !(qw - kb - 31 < a.W || kb < a.sinks)) continue;
+      f32x16 s = R::rows(Ks + 32 * sub * R::P, qf, lane);
+      const f32x16 dp = R::rows(Vs + 32 * sub * R::P, df, lane);
+      const uint32_t bits =
+          (uint32_t)__ballot(kb + (lane & 31) < a.S && (!mask || mask[kb + (lane & 31)])) >> (4 * hh);
+      const bool all = !__any(bits != (hh ? 0x0fffffffu : 0xffffffffu)) && kb + 31 <= qw &&
+                       (qw + 31 - kb < a.W || kb + 31 < a.sinks);
+      const bool near = BIAS && qw - kb - 31 < a.maxd;
+      if (BIAS) {
+        if (near) {
+          const float* at = lut + kLutOff + qi - kb - 4 * hh;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, at[-kappa(r)] - L);
+        } else {
+          const float b = lut[lut_size(a.maxd) - 1] - L;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, b);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, -L);
+      }
+      float ds[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(s[r]) * (dp[r] - Dq);
+      if (!all) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = kb + kappa(r) + 4 * hh;
+          const bool see = key <= qi && (qi - key < a.W || key < a.sinks) && ((bits >> kappa(r)) & 1);
+          ds[r] = see ? ds[r] : 0.f;
+        }
+      }
+      R::cols(acc, Ks + 32 * sub * R::P, ds, lane);
+      if (BIAS) {
+        if (near) {
+          float* at = sk_w + (lane & 31) * 65 + 31 - 4 * hh;       // row i, column i − key + 31
+#pragma unroll
+          for (int r = 0; r < 16; ++r) at[-kappa(r)] = ds[r];
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sum += sk_w[i * 64 + lane];
+          const int d = qw - kb + lane - 31;
+          if (lane < 63 && d >= 0) bins[d] += sum;
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) far += ds[r];
+        }
+      }
+    }
+  }
+  if (qi < a.S) {
+    T* out = (T*)a.dq + (tok0 + qi) * (int64_t)(a.H * D) + h * D + 4 * hh;
+#pragma unroll
+    for (int db = 0; db < R::DB; ++db)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        Elem<T>::store4(out + 32 * db + 8 * c, acc[db][4 * c] * a.scale, acc[db][4 * c + 1] * a.scale,
+                        acc[db][4 * c + 2] * a.scale, acc[db][4 * c + 3] * a.scale);
+  }
+  if (BIAS) {
+    far = wave_sum(far);
+    if (lane == 0) fars[w] = far;
+    __syncthreads();
+    float* out = a.bpart + (((int64_t)n * a.H + h) * nqt + qt) * a.NB;
+    for (int b = w; b < a.NB; b += NW) {
+      const int end = b + 1 < a.NB ? a.start[b + 1] : nbin;
+      float sum = 0.f;
+      for (int d = a.start[b] + lane; d < end; d += 64)
+#pragma unroll
+        for (int i = 0; i < NW; ++i) sum += lut[lut_size(a.maxd) + i * nbin + d];
+      sum = wave_sum(sum);
+      if (b == a.NB - 1)
+#pragma unroll
+        for (int i = 0; i < NW; ++i) sum += fars[i];
+      if (lane == 0) out[b] = sum;
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------------------
+// Backward, dk and dv: a wave owns 32 keys (its columns), the workgroup 32·NW of one kv head; it walks the queries
+// that see them through the window, for every query head of the kv head. The first workgroups are the sink pass: what
+// the sinks get from queries beyond the window, a chunk of queries each, as partial sums that finish_kernel adds up in
+// order (the sinks' own rows of the window pass among them).
+// ----------------------------------------------------------------------------------------------------------------
+template <typename T, int D, int NW, int BQ>
+__global__ __launch_bounds__(64 * NW) void dkv_kernel(const Args a) {
+  using R = Row<T, D>;
+  __shared__ __attribute__((aligned(16))) T Qs[BQ * R::P];
+  __shared__ __attribute__((aligned(16))) T Os[BQ * R::P];
+  __shared__ __attribute__((aligned(16))) float Ls[BQ], Ds[BQ];
+  extern __shared__ float lut[];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
+  const int G = a.H / a.KV, nkt = (a.S + 32 * NW - 1) / (32 * NW);
+  const int nsink = a.nchunk * a.N * a.KV;
+  const bool sink = (int)blockIdx.x < nsink;
+  int id = sink ? (int)blockIdx.x : xcd_swizzle(blockIdx.x - nsink, gridDim.x - nsink);
+  const int kt = sink ? 0 : id % nkt, chunk = sink ? id % a.nchunk : 0;
+  id /= sink ? a.nchunk : nkt;
+  const int kv = id % a.KV, n = id / a.KV;
+  const int64_t tok0 = (int64_t)n * a.S;
+  const uint8_t* mask = a.mask ? a.mask + tok0 : nullptr;
+  const int k0 = kt * 32 * NW, kw = k0 + 32 * w, kj = kw + (lane & 31);
+  const bool real = kj < a.S && (!mask || mask[kj]) && (!sink || kj < a.sinks);
+  uint4 kf[R::NC], vf[R::NC];
+  R::frags(kf, (const T*)a.k + (tok0 + kj) * a.ldk + kv * D, real, hh);
+  R::frags(vf, (const T*)a.v + (tok0 + kj) * a.ldv + kv * D, real, hh);
+  // queries [qs, qe): through the window, or a chunk of those beyond it
+  int qs, qe;
+  if (sink) {
+    qs = a.W + chunk * a.qchunk;
+    qe = qs + a.qchunk < a.S ? qs + a.qchunk : a.S;
+  } else {
+    qs = k0;
+    qe = (int64_t)k0 + 32 * NW - 1 + a.W < a.S ? k0 + 32 * NW - 1 + a.W : a.S;
+  }
+  const int nt = (qe - qs + BQ - 1) / BQ;
+  const bool allreal = !__any(!real);
+  const int count = __syncthreads_or(real) ? nt * G : 0;
+  const float c2 = a.scale * kLog2e;
+  f32x16 ak[R::DB], av[R::DB];
+#pragma unroll
+  for (int db = 0; db < R::DB; ++db) ak[db] = av[db] = zero16();
+  Stage<T, D, BQ, 64 * NW> sq, so;
+  float sl = 0.f, sd = 0.f;                        // threads below BQ: the row's statistics
+  auto load = [&](int it) {
+    const int h = kv * G + it / nt, q0 = qs + (it % nt) * BQ;
+    sq.load((const T*)a.q + tok0 * a.ldq + h * D, a.ldq, q0, qe, mask, tid);
+    so.load((const T*)a.dout + tok0 * a.lddo + h * D, a.lddo, q0, qe, mask, tid);
+    if (tid < BQ) {
+      const int64_t at = ((int64_t)n * a.H + h) * a.S + q0 + tid;
+      sl = q0 + tid < qe ? a.lse[at] : INFINITY;   // a masked query's is +inf, its D zero
+      sd = q0 + tid < qe ? a.dsum[at] : 0.f;
+    }
+  };
+  if (count) load(0);
+  for (int it = 0; it < count; ++it) {
+    const int q0 = qs + (it % nt) * BQ;
+    __syncthreads();
+    sq.store(Qs, tid);
+    so.store(Os, tid);
+    if (tid < BQ) {
+      Ls[tid] = sl;
+      Ds[tid] = sd;
+    }
+    if (a.bias && it % nt == 0) fill_lut(lut, a, n / (a.N / a.C), kv * G + it / nt, tid, 64 * NW);
+    __syncthreads();
+    if (it + 1 < count) load(it + 1);
+#pragma unroll
+    for (int sub = 0; sub < BQ / 32; ++sub) {
+      const int qb = q0 + 32 * sub;
+      if (kw >= a.S || qb >= qe || qb + 31 < kw) continue;
+      if (sink ? (kw >= a.sinks || qb + 31 - kw < a.W) : qb - kw - 31 >= a.W) continue;
+      const bool all = allreal && (sink ? qb - kw - 31 >= a.W : qb >= kw + 31 && qb + 31 - kw < a.W);
+      f32x16 s = R::rows(Qs + 32 * sub * R::P, kf, lane);
+      const f32x16 dp = R::rows(Os + 32 * sub * R::P, vf, lane);
+      if (a.bias) {
+        if (qb - kw - 31 < a.maxd) {
+          const float* at = lut + kLutOff + qb - kj + 4 * hh;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, at[kappa(r)]);
+        } else {
+          const float far = lut[lut_size(a.maxd) - 1];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, far);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= c2;
+      }
+      float p[16], ds[16];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float4 L4 = *reinterpret_cast<const float4*>(Ls + 32 * sub + 8 * c + 4 * hh);
+        const float4 D4 = *reinterpret_cast<const float4*>(Ds + 32 * sub + 8 * c + 4 * hh);
+        const float Lr[4] = {L4.x, L4.y, L4.z, L4.w}, Dr[4] = {D4.x, D4.y, D4.z, D4.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          p[4 * c + j] = __builtin_amdgcn_exp2f(s[4 * c + j] - Lr[j]);
+          ds[4 * c + j] = p[4 * c + j] * (dp[4 * c + j] - Dr[j]);
+        }
+      }
+      if (!all) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int d = qb + kappa(r) + 4 * hh - kj;
+          const bool see = real && d >= 0 && (sink ? d >= a.W : d < a.W);
+          p[r] = see ? p[r] : 0.f;
+          ds[r] = see ? ds[r] : 0.f;
+        }
+      }
+      R::cols(av, Os + 32 * sub * R::P, p, lane);
+      R::cols(ak, Qs + 32 * sub * R::P, ds, lane);
+    }
+  }
+  if (kj >= a.S || (sink && kj >= a.sinks)) return;
+  if (a.nchunk && kj < a.sinks) {
+    float* pk = a.part + ((((int64_t)n * a.KV + kv) * (a.nchunk + 1) + (sink ? chunk + 1 : 0)) * 2 * a.sinks + kj) * D +
+                4 * hh;
+    float* pv = pk + (int64_t)a.sinks * D;
+#pragma unroll
+    for (int db = 0; db < R::DB; ++db)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        Elem<float>::store4(pk + 32 * db + 8 * c, ak[db][4 * c] * a.scale, ak[db][4 * c + 1] * a.scale,
+                            ak[db][4 * c + 2] * a.scale, ak[db][4 * c + 3] * a.scale);
+        Elem<float>::store4(pv + 32 * db + 8 * c, av[db][4 * c], av[db][4 * c + 1], av[db][4 * c + 2],
+                            av[db][4 * c + 3]);
+      }
+    return;
+  }
+  const int64_t at = (tok0 + kj) * (int64_t)(a.KV * D) + kv * D + 4 * hh;
+#pragma unroll
+  for (int db = 0; db < R::DB; ++db)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      Elem<T>::store4((T*)a.dk + at + 32 * db + 8 * c, ak[db][4 * c] * a.scale, ak[db][4 * c + 1] * a.scale,
+                      ak[db][4 * c + 2] * a.scale, ak[db][4 * c + 3] * a.scale);
+      Elem<T>::store4((T*)a.dv + at + 32 * db + 8 * c, av[db][4 * c], av[db][4 * c + 1], av[db][4 * c + 2],
+                      av[db][4 * c + 3]);
+    }
+}
+
+// The partial sums' last step, in a fixed order. Workgroups [0, C·H): dbias of a client and head over its sequences and
+// query tiles (in fp64: dS sums to zero over a row, so buckets are small next to their terms); the others: the sinks'
+// rows of dk and dv.
+template <typename T>
+__global__ __launch_bounds__(256) void finish_kernel(const Args a, int D, int nqt) {
+  __shared__ double red[256];
+  const int nb = a.dbias ? a.C * a.H : 0;
+  if ((int)blockIdx.x < nb) {
+    const int c = blockIdx.x / a.H, h = blockIdx.x % a.H, per = a.N / a.C;
+    int wide = 1;
+    while (wide < a.NB) wide *= 2;
+    const int b = threadIdx.x % wide, row = threadIdx.x / wide, rows = 256 / wide;
+    double sum = 0.;
+    if (b < a.NB)
+      for (int64_t i = row; i < (int64_t)per * nqt; i += rows)
+        sum += a.bpart[((((int64_t)c * per + i / nqt) * a.H + h) * nqt + i % nqt) * a.NB + b];
+    red[threadIdx.x] = sum;
+    __syncthreads();
+    if (row == 0 && b < a.NB) {
+      for (int i = 1; i < rows; ++i) sum += red[i * wide + b];
+      a.dbias[((int64_t)c * a.H + h) * a.NB + b] = (float)sum;
+    }
+    return;
+  }
+  const int64_t e = ((int64_t)blockIdx.x - nb) * 256 + threadIdx.x;       // [n][kv][dk | dv][sink][D / 4]
+  const int64_t one = (int64_t)2 * a.sinks * (D / 4);
+  if (e >= (int64_t)a.N * a.KV * one) return;
+  const int64_t head = e / one;
+  const int in = (int)(e % one);
+  const float4* p = reinterpret_cast<const float4*>(a.part) + head * (a.nchunk + 1) * one + in;
+  float4 s = p[0];
+  for (int i = 1; i <= a.nchunk; ++i) {
+    const float4 x = p[i * one];
+    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+  }
+  const int which = in / (a.sinks * (D / 4)), rest = in % (a.sinks * (D / 4)), j = rest / (D / 4);
+  const int64_t n = head / a.KV, kv = head % a.KV;
+  T* out = (T*)(which ? a.dv : a.dk) + (n * a.S + j) * (a.KV * D) + kv * D + 4 * (rest % (D / 4));
+  if (j < a.S) Elem<T>::store4(out, s.x, s.y, s.z, s.w);
+}
+
+// ----------------------------------------------------------------------------------------------------------------
+// One new token per sequence over a ring cache [batch][sinks + W][KV·D]: slot s < sinks holds token s, slot
+// sinks + (t − sinks) mod W token t. The query heads of a kv head are the columns; a wave reads 32 slots at a time
+// into an LDS tile of its own (the next 32 in flight in registers), keeps its own softmax, and the workgroup's waves,
+// then the splits of the cache, are joined by their maxima. The new token's rows are taken from the arguments, and
+// written into their slot by the workgroup that reads them.
+// ----------------------------------------------------------------------------------------------------------------
+struct StepArgs {
+  const void *q, *k, *v;
+  void *kc, *vc, *o;
+  const int* pos;
+  const float* bias;
+  float *pacc, *pml;             // splits > 1: [B·H][splits][D], [B·H][splits][2]
+  int64_t ldq, ldk, ldv;
+  int B, H, KV, C, W, sinks, NB, maxd, splits, per;   // per: slots of a split, a multiple of 32
+  float scale;
+  int start[kMaxBuckets];
+};
+
+// the age (pos − token) of the token in a slot, −1 if there is none; cur = the new token's slot
+__device__ __forceinline__ int slot_age(int s, int pos, int sinks, int W, int cur) {
+  if (pos < 0) return -1;
+  if (s < sinks) return s <= pos ? pos - s : -1;
+  if (pos < sinks) return -1;
+  int age = cur - s;
+  if (age < 0) age += W;
+  return pos - age >= sinks ? age : -1;
+}
+
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW) void step_kernel(const StepArgs a) {
+  using R = Row<T, D>;
+  __shared__ __attribute__((aligned(16))) T tiles[NW][2][32 * R::P];
+  __shared__ float ml[NW][2][32];
+  extern __shared__ float tab[];                  // bias: [heads of the group][NB], then bytes: bucket of a distance
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
+  const int G = a.H / a.KV, groups = (G + 31) / 32;
+  int id = blockIdx.x;
+  const int split = id % a.splits;
+  id /= a.splits;
+  const int grp = id % groups;
+  id /= groups;
+  const int kv = id % a.KV, b = id / a.KV;
+  const int n = a.sinks + a.W, pos = a.pos[b];
+  const int cur = pos < a.sinks ? pos : a.sinks + (pos - a.sinks) % a.W;
+  const int g = grp * 32 + (lane & 31), h = kv * G + g;
+  const bool real = g < G;
+  uint8_t* of = reinterpret_cast<uint8_t*>(tab + 32 * a.NB);
+  if (a.bias) {
+    const float* src = a.bias + ((int64_t)(b / (a.B / a.C)) * a.H + kv * G + grp * 32) * a.NB;
+    const int have = (G - grp * 32 < 32 ? G - grp * 32 : 32) * a.NB;
+    for (int i = tid; i < 32 * a.NB; i += 64 * NW) tab[i] = i < have ? src[i] * kLog2e : 0.f;
+    for (int d = tid; d <= a.maxd; d += 64 * NW) {
+      int x = 0;
+      for (int i = 1; i < a.NB; ++i) x += d >= a.start[i] ? 1 : 0;
+      of[d] = (uint8_t)x;
+    }
+  }
+  __syncthreads();
+  uint4 qf[R::NC];
+  R::frags(qf, (const T*)a.q + b * a.ldq + (int64_t)h * D, real, hh);
+  T* kc = (T*)a.kc + (int64_t)b * n * a.KV * D + kv * D;
+  T* vc = (T*)a.vc + (int64_t)b * n * a.KV * D + kv * D;
+  const T* kn = (const T*)a.k + b * a.ldk + kv * D;
+  const T* vn = (const T*)a.v + b * a.ldv + kv * D;
+  const int ld = a.KV * D;
+  const int s0 = split * a.per, s1 = s0 + a.per < n ? s0 + a.per : n;
+  constexpr int NI = 32 * R::U / 64;
+  uint4 rk[NI], rv[NI];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int u = lane + 64 * i, s = base + u / R::U, c = (u % R::U) * R::E;
+      rk[i] = rv[i] = make_uint4(0, 0, 0, 0);
+      if (s >= s1 || slot_age(s, pos, a.sinks, a.W, cur) < 0) continue;
+      if (s == cur) {
+        rk[i] = *reinterpret_cast<const uint4*>(kn + c);
+        rv[i] = *reinterpret_cast<const uint4*>(vn + c);
+        if (grp == 0) {
+          *reinterpret_cast<uint4*>(kc + (int64_t)s * ld + c) = rk[i];
+          *reinterpret_cast<uint4*>(vc + (int64_t)s * ld + c) = rv[i];
+        }
+      } else {
+        rk[i] = *reinterpret_cast<const uint4*>(kc + (int64_t)s * ld + c);
+        rv[i] = *reinterpret_cast<const uint4*>(vc + (int64_t)s * ld + c);
+      }
+    }
+  };
+  const float c2 = a.scale * kLog2e;
+  float m = -INFINITY, l = 0.f;
+  f32x16 acc[R::DB];
+#pragma unroll
+  for (int db = 0; db < R::DB; ++db) acc[db] = zero16();
+  T *Ks = tiles[w][0], *Vs = tiles[w][1];
+  if (pos >= 0) {
+    int base = s0 + 32 * w;
+    if (base < s1) load(base);
+    for (; base < s1; base += 32 * NW) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int u = lane + 64 * i;
+        *reinterpret_cast<uint4*>(Ks + (u / R::U) * R::P + (u % R::U) * R::E) = rk[i];
+        *reinterpret_cast<uint4*>(Vs + (u / R::U) * R::P + (u % R::U) * R::E) = rv[i];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (base + 32 * NW < s1) load(base + 32 * NW);
+      f32x16 s = R::rows(Ks, qf, lane);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int slot = base + kappa(r) + 4 * hh;
+        const int age = slot < s1 ? slot_age(slot, pos, a.sinks, a.W, cur) : -1;
+        float x = s[r] * c2;
+        if (a.bias && age >= 0) x += tab[(lane & 31) * a.NB + of[age < a.maxd ? age : a.maxd]];
+        s[r] = age >= 0 ? x : -INFINITY;
+      }
+      float mt = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
+      mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+      const float mn = fmaxf(m, mt), mu = mn == -INFINITY ? 0.f : mn;
+      const float al = __builtin_amdgcn_exp2f(m - mu);
+      l *= al;
+#pragma unroll
+      for (int db = 0; db < R::DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[db][r] *= al;
+      m = mn;
+      float p[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        p[r] = __builtin_amdgcn_exp2f(s[r] - mu);
+        l += p[r];
+      }
+      R::cols(acc, Vs, p, lane);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (hh == 0) {
+    ml[w][0][lane] = m;
+    ml[w][1][lane] = l;
+  }
+  // the waves' sums, scaled to the common maximum, through their own tiles
+  float* mine = reinterpret_cast<float*>(tiles[w]);
+  static_assert(2 * 32 * R::P * sizeof(T) >= 32 * D * sizeof(float), "the tiles hold a wave's sums");
+  __syncthreads();
+  float M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) M = fmaxf(M, ml[i][0][lane & 31]);
+  const float Mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) L += ml[i][1][lane & 31] * __builtin_amdgcn_exp2f(ml[i][0][lane & 31] - Mu);
+  const float al = __builtin_amdgcn_exp2f(m - Mu);
+#pragma unroll
+  for (int db = 0; db < R::DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mine[(lane & 31) * D + 32 * db + kappa(r) + 4 * hh] = acc[db][r] * al;
+  __syncthreads();
+  // a column (head) of D sums at a time
+  const int heads = G - grp * 32 < 32 ? G - grp * 32 : 32;
+  for (int e = tid * 4; e < heads * D; e += 64 * NW * 4) {
+    float4 s = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(tiles[0]) + e);
+#pragma unroll
+    for (int i = 1; i < NW; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(tiles[i]) + e);
+      s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+    }
+    const int hd = e / D, d = e % D;
+    const int64_t row = (int64_t)b * a.H + kv * G + grp * 32 + hd;
+    if (a.splits > 1) {
+      Elem<float>::store4(a.pacc + (row * a.splits + split) * D + d, s.x, s.y, s.z, s.w);
+    } else {
+      float Mh = -INFINITY, Lh = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) Mh = fmaxf(Mh, ml[i][0][hd]);
+#pragma unroll
+      for (int i = 0; i < NW; ++i)
+        Lh += ml[i][1][hd] * __builtin_amdgcn_exp2f(ml[i][0][hd] - (Mh == -INFINITY ? 0.f : Mh));
+      const float inv = Lh == 0.f ? 0.f : 1.f / Lh;
+      Elem<T>::store4((T*)a.o + row * D + d, s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+    }
+  }
+  if (a.splits > 1 && w == 0 && lane < heads) {
+    float* out = a.pml + (((int64_t)b * a.H + kv * G + grp * 32 + lane) * a.splits + split) * 2;
+    out[0] = M;
+    out[1] = L;
+  }
+}
+
+// joins the splits of a (sequence, head): one wave each
+template <typename T, int D>
+__global__ __launch_bounds__(64) void step_join_kernel(const StepArgs a) {
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  float M = -INFINITY;
+  for (int i = lane; i < a.splits; i += 64) M = fmaxf(M, a.pml[(row * a.splits + i) * 2]);
+  M = wave_max(M);
+  const float Mu = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  for (int i = lane; i < a.splits; i += 64)
+    L += a.pml[(row * a.splits + i) * 2 + 1] * __builtin_amdgcn_exp2f(a.pml[(row * a.splits + i) * 2] - Mu);
+  L = wave_sum(L);
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  for (int d = lane; d < D; d += 64) {
+    float s = 0.f;
+    for (int i = 0; i < a.splits; ++i)
+      s += a.pacc[(row * a.splits + i) * D + d] * __builtin_amdgcn_exp2f(a.pml[(row * a.splits + i) * 2] - Mu);
+    if constexpr (sizeof(T) == 2) ((T*)a.o)[row * D + d] = f32_to_bf16(s * inv);
+    else ((T*)a.o)[row * D + d] = s * inv;
+  }
+}
+
+// a prompt's rows into the cache: what the slots hold after token len − 1; slots of no token stay as they were
+__global__ __launch_bounds__(256) void fill_kernel(const uint4* __restrict__ k, const uint4* __restrict__ v,
+                                                   int64_t ldk, int64_t ldv, uint4* __restrict__ kc,
+                                                   uint4* __restrict__ vc, const int* __restrict__ lengths, int B,
+                                                   int S, int W, int sinks, int U) {
+  const int n = sinks + W;
+  const int64_t total = (int64_t)B * n * U;
+  for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
+    const int u = (int)(e % U), s = (int)(e / U % n), b = (int)(e / U / n);
+    int len = lengths ? lengths[b] : S;
+    len = len < 0 ? 0 : len > S ? S : len;
+    const int pos = len - 1, cur = pos < sinks ? pos : sinks + (pos - sinks) % W;
+    const int age = slot_age(s, pos, sinks, W, cur);
+    if (age < 0) continue;
+    const int64_t row = (int64_t)b * S + pos - age;
+    kc[e] = k[row * ldk + u];
+    vc[e] = v[row * ldv + u];
+  }
+}
+
+template <typename T, int D, int NW, int BK> int launch_fwd_tile(const Args& a, hipStream_t st) {
+  const size_t lds = a.bias ? (a.maxd + 2 * kLutOff) * sizeof(float) : 0;
+  const dim3 grid((unsigned)((int64_t)a.N * a.H * ((a.S + 32 * NW - 1) / (32 * NW)))), block(64 * NW);
+  if (sizeof(T) == 2 && a.olo) hipLaunchKernelGGL((fwd_kernel<T, D, NW, BK, sizeof(T) == 2>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((fwd_kernel<T, D, NW, BK, false>), grid, block, lds, st, a);
+  return (int)hipGetLastError();
+}
+
+template <typename T, int D> int launch_fwd(const Args& a, hipStream_t st) {
+  if (a.S > 64) return launch_fwd_tile<T, D, 4, sizeof(T) == 2 ? 64 : 32>(a, st);
+  return launch_fwd_tile<T, D, 1, 32>(a, st);
+}
+
+template <typename T, int D, int NW, int BK> int launch_dq(const Args& a, hipStream_t st) {
+  const int64_t n = (int64_t)a.N * a.H * ((a.S + 32 * NW - 1) / (32 * NW));
+  if (a.dbias) {
+    const size_t lds = (a.maxd + 2 * kLutOff + NW * (a.maxd + kBinPad)) * sizeof(float);
+    hipLaunchKernelGGL((dq_kernel<T, D, NW, BK, true>), dim3((unsigned)n), dim3(64 * NW), lds, st, a);
+  } else {
+    hipLaunchKernelGGL((dq_kernel<T, D, NW, BK, false>), dim3((unsigned)n), dim3(64 * NW), 0, st, a);
+  }
+  return (int)hipGetLastError();
+}
+
+template <typename T, int D> int launch_bwd(const Args& a, hipStream_t st) {
+  const size_t lds = a.bias ? (a.maxd + 2 * kLutOff) * sizeof(float) : 0;
+  int rc;
+  if (a.S > 64) rc = launch_dq<T, D, 4, 32>(a, st);
+  else rc = launch_dq<T, D, 1, 32>(a, st);
+  if (rc) return rc;
+  const int64_t nsink = (int64_t)a.nchunk * a.N * a.KV;
+  // 64 keys suffice for a short sequence; at fp32 and 128 dims two waves would have to spill
+  constexpr int kFew = D * sizeof(T) > 256 ? 4 : 2;
+  if (a.S > 64) {
+    const int64_t n = nsink + (int64_t)a.N * a.KV * ((a.S + 127) / 128);
+    hipLaunchKernelGGL((dkv_kernel<T, D, 4, 32>), dim3((unsigned)n), dim3(256), lds, st, a);
+  } else {
+    const int64_t n = nsink + (int64_t)a.N * a.KV;
+    hipLaunchKernelGGL((dkv_kernel<T, D, kFew, 32>), dim3((unsigned)n), dim3(64 * kFew), lds, st, a);
+  }
+  if ((rc = (int)hipGetLastError())) return rc;
+  const int nqt = a.S > 64 ? (a.S + 127) / 128 : (a.S + 31) / 32;
+  const int64_t blocks = (a.dbias ? (int64_t)a.C * a.H : 0) +
+                         (a.nchunk ? ((int64_t)a.N * a.KV * 2 * a.sinks * (D / 4) + 255) / 256 : 0);
+  if (blocks) hipLaunchKernelGGL(finish_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, a, D, nqt);
+  return (int)hipGetLastError();
+}
+
+template <typename T, int D> int launch_step(const StepArgs& a, hipStream_t st) {
+  constexpr int NW = D * sizeof(T) > 256 ? 2 : 4;
+  const size_t lds = a.bias ? 32 * a.NB * sizeof(float) + (a.maxd + 4) / 4 * 4 : 0;
+  const int64_t n = (int64_t)a.B * a.KV * ((a.H / a.KV + 31) / 32) * a.splits;
+  hipLaunchKernelGGL((step_kernel<T, D, NW>), dim3((unsigned)n), dim3(64 * NW), lds, st, a);
+  int rc = (int)hipGetLastError();
+  if (rc || a.splits == 1) return rc;
+  hipLaunchKernelGGL((step_join_kernel<T, D>), dim3((unsigned)(a.B * a.H)), dim3(64), 0, st, a);
+  return (int)hipGetLastError();
+}
+
+}  // namespace win
+
+#define FA_WIN_DISPATCH(FN, A, ST)                                             \
+  if (bf16 && D == 64) return win::FN<uint16_t, 64>(A, ST);                    \
+  if (bf16 && D == 128) return win::FN<uint16_t, 128>(A, ST);                  \
+  if (!bf16 && D == 64) return win::FN<float, 64>(A, ST);                      \
+  if (!bf16 && D == 128) return win::FN<float, 128>(A, ST);                    \
+  return (int)hipErrorInvalidValue;
+
+FA_EXPORT int fa_window_fwd(const win::Args* a, int bf16, int D, hipStream_t stream) {
+  FA_WIN_DISPATCH(launch_fwd, *a, stream)
+}
+FA_EXPORT int fa_window_bwd(const win::Args* a, int bf16, int D, hipStream_t stream) {
+  FA_WIN_DISPATCH(launch_bwd, *a, stream)
+}
+FA_EXPORT int fa_window_step(const win::StepArgs* a, int bf16, int D, hipStream_t stream) {
+  FA_WIN_DISPATCH(launch_step, *a, stream)
+}
+FA_EXPORT int fa_window_fill(const void* k, const void* v, int64_t ldk, int64_t ldv, void* kc, void* vc,
+                             const int* lengths, int B, int S, int W, int sinks, int U, hipStream_t stream) {
+  const int64_t n = (int64_t)B * (sinks + W) * U;
+  hipLaunchKernelGGL(win::fill_kernel, dim3(fa_grid(n, 256, 16384)), dim3(256), 0, stream, (const uint4*)k,
+                     (const uint4*)v, ldk, ldv, (uint4*)kc, (uint4*)vc, lengths, B, S, W, sinks, U);
+  return (int)hipGetLastError();
+}

@@ -1,0 +1,167 @@
+"""Gated linear recurrence over long sequences (``csrc/scan_kernels.hip``): per sequence and feature
+
+    f_t = σ(gate_t),   h_t = f_t·h_{t−1} + (1 − f_t)·x_t,   y_t = h_t
+
+The recurrence is linear in the state, so unlike an LSTM's (:mod:`.rnn_ops`) it needs no product with a weight per step
+and a whole sequence is ONE launch each way. Layout of the recurrent models: ``[C, T, B, H]`` (client, time, sequence,
+feature); any strides with dense features, so token-major rows go in as ``x.view(C, B, T, H).transpose(1, 2)``.
+
+CUDA tensors run the HIP kernels (bf16 or fp32 storage; states, maps and sums fp32), CPU tensors the same recurrence in
+plain PyTorch (fp64 for fp64 inputs), the tests' oracle. Results are the same bit for bit from call to call. Everything
+is enqueued on the current stream of the tensors' device and may be captured into a HIP graph."""
+import ctypes as _c
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .fl_ops import _check, _fn, _p, _pr, _stream, use_native
+
+_TILE = 64                # steps between two kept states
+_I32 = 2 ** 31 - 1
+
+
+class _Args(_c.Structure):
+    _fields_ = [(n, _c.c_void_p) for n in ("x", "gate", "dy", "y", "dx", "dgate", "h0", "dh", "hT", "dh0", "ckpt",
+                                           "agg", "mask")] + \
+               [(n, _c.c_int64 * 3) for n in ("xs", "gs", "dys", "ys", "ms")] + \
+               [(n, _c.c_int) for n in ("C", "T", "B", "H", "nseg", "tps")]
+
+
+def _v(p):
+    return None if p is None else p.value
+
+
+def _dense(t):
+    """Dense features; nothing else is asked of the strides."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _like(x):
+    """An empty [C, T, B, H] laid out in x's order of time and sequence."""
+    C, T, B, H = x.shape
+    if x.stride(2) > x.stride(1):
+        return torch.empty(C, B, T, H, dtype=x.dtype, device=x.device).transpose(1, 2)
+    return torch.empty(C, T, B, H, dtype=x.dtype, device=x.device)
+
+
+def _launch(a, x, gate, mask, streams, bwd):
+    C, T, B, H = x.shape
+    a.C, a.T, a.B, a.H = C, T, B, H
+    a.x, a.gate, a.mask = _v(_pr(x)), _v(_pr(gate)), _v(_pr(mask))
+    a.xs[:], a.gs[:] = x.stride()[:3], gate.stride()[:3]
+    if mask is not None:
+        a.ms[:] = mask.stride()
+    vec = 2
+    for t in (x, gate, *streams):       # two features at a time where every row starts at a multiple of two
+        if H % 2 or t.data_ptr() % (2 * t.element_size()) or any(s % 2 for s in t.stride()[:3]):
+            vec = 1
+    wgs, ntile = C * B * -(-H // (32 * vec)), -(-T // _TILE)
+    nseg = 1 if wgs >= 512 else min(ntile, -(-1024 // wgs), 64)
+    a.tps = -(-ntile // nseg)
+    a.nseg = -(-ntile // a.tps)
+    if wgs * a.nseg > _I32:
+        raise ValueError(f"gated_scan: {C} clients · {B} sequences · {H} features are too many for one call")
+    agg = None
+    if a.nseg > 1:
+        agg = torch.empty(C * B * a.nseg * 2 * H, dtype=torch.float32, device=x.device)
+        a.agg = _v(_p(agg))
+    with torch.cuda.device(x.device):
+        _check(_fn("fa_gated_scan")(_c.byref(a), _c.c_int(int(x.dtype == torch.bfloat16)), _c.c_int(vec),
+                                    _c.c_int(int(bwd)), _stream(x)), "fa_gated_scan")
+
+
+def _forward(x, gate, h0, mask, keep):
+    C, T, B, H = x.shape
+    y = _like(x)
+    hT = torch.empty(C, B, H, dtype=torch.float32, device=x.device)
+    ckpt = torch.empty(C, -(-T // _TILE), B, H, dtype=torch.float32, device=x.device) if keep else None
+    if y.numel():
+        a = _Args(y=_v(_p(y)), hT=_v(_p(hT)), h0=_v(_pr(h0)), ckpt=_v(_p(ckpt)))
+        a.ys[:] = y.stride()[:3]
+        _launch(a, x, gate, mask, (y,), False)
+    return y, hT, ckpt
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, h0, mask):
+        x, gate = _dense(x), _dense(gate)
+        y, hT, ckpt = _forward(x, gate, None if h0 is None else h0.contiguous(), mask, True)
+        ctx.save_for_backward(x, gate, mask, ckpt)
+        ctx.set_materialize_grads(False)
+        return y, hT
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        x, gate, mask, ckpt = ctx.saved_tensors
+        if dy is None and dh is None:
+            return None, None, None, None
+        C, T, B, H = x.shape
+        dy = torch.zeros_like(x) if dy is None else _dense(dy.to(x.dtype))
+        dh = None if dh is None else dh.contiguous()
+        dx, dgate = _like(x), _like(x)
+        dh0 = torch.empty(C, B, H, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
+        if dx.numel():
+            a = _Args(dy=_v(_pr(dy)), dh=_v(_pr(dh)), dx=_v(_p(dx)), dgate=_v(_p(dgate)), dh0=_v(_p(dh0)),
+                      ckpt=_v(_pr(ckpt)))
+            a.ys[:], a.dys[:] = dx.stride()[:3], dy.stride()[:3]
+            _launch(a, x, gate, mask, (dx, dgate, dy), True)
+        return dx, dgate, dh0, None
+
+
+def _scan_ref(x, gate, h0, mask):
+    ct = torch.float64 if x.dtype == torch.float64 else torch.float32
+    C, T, B, H = x.shape
+    g, b = gate.to(ct), x.to(ct)
+    real = None if mask is None else (mask != 0).unsqueeze(-1)
+    zero = torch.zeros((), dtype=ct, device=x.device)
+    if real is not None:      # selected before any product: what padding holds reaches nothing
+        g, b = torch.where(real, g, zero), torch.where(real, b, zero)
+    ls = torch.nn.functional.logsigmoid       # f and 1 − f by their logarithms: neither they nor their slopes cancel
+    f, b = ls(g).exp(), ls(-g).exp() * b
+    if real is not None:
+        f = torch.where(real, f, zero + 1)
+    h = torch.zeros(C, B, H, dtype=ct, device=x.device) if h0 is None else h0.to(ct)
+    ys = []
+    for t in range(T):
+        h = f[:, t] * h + b[:, t]
+        ys.append(h if real is None else torch.where(real[:, t], h, zero))
+    return torch.stack(ys, 1).to(x.dtype), h
+
+
+def gated_scan(x: torch.Tensor, gate: torch.Tensor, h0: torch.Tensor = None, mask: torch.Tensor = None):
+    """(y, h_T) of the recurrence above for ``x`` and ``gate`` [C, T, B, H] from the state ``h0`` [C, B, H] (fp32; zero
+    if not given): y [C, T, B, H] at x's type, in x's order of time and sequence, and the state after the last step
+    h_T [C, B, H], fp32 — the ``h0`` of the next call. T = 1 is the step of a program that answers token by token.
+
+    ``mask`` [C, T, B] (bool or integer, nonzero = a step): a step that is padding leaves the state as it is, its y is
+    zero, and what x, gate and the gradient of y hold there (NaN included) reaches nothing. Gradients: x, gate (at their
+    type) and h0 (fp32)."""
+    if x.dim() != 4 or gate.shape != x.shape:
+        raise ValueError(f"gated_scan: x and gate [C, T, B, H] expected, got {tuple(x.shape)} and {tuple(gate.shape)}")
+    if x.dtype not in (torch.bfloat16, torch.float32) and (x.is_cuda or x.dtype != torch.float64):
+        raise TypeError(f"gated_scan: bf16 or fp32 expected, got {x.dtype}")
+    if gate.dtype != x.dtype or gate.device != x.device:
+        raise TypeError(f"gated_scan: gate is {gate.dtype} on {gate.device}, x {x.dtype} on {x.device}")
+    C, T, B, H = x.shape
+    if T < 1 or H < 1:
+        raise ValueError(f"gated_scan: at least one step and one feature expected, got {tuple(x.shape)}")
+    if T > _I32 - 2 * _TILE:
+        raise ValueError(f"gated_scan: {T} steps are too many for one call")
+    state = torch.float64 if x.dtype == torch.float64 else torch.float32
+    if h0 is not None and (h0.shape != (C, B, H) or h0.dtype != state or h0.device != x.device):
+        raise ValueError(f"gated_scan: h0 {state} [{C}, {B}, {H}] on {x.device} expected, got {h0.dtype} "
+                         f"{tuple(h0.shape)} on {h0.device}")
+    if mask is not None and (mask.shape != (C, T, B) or mask.dtype.is_floating_point or mask.dtype.is_complex or
+                             mask.device != x.device):
+        raise ValueError(f"gated_scan: mask bool or integer [{C}, {T}, {B}] on {x.device} expected, got {mask.dtype} "
+                         f"{tuple(mask.shape)} on {mask.device}")
+    if not use_native(x):
+        return _scan_ref(x, gate, h0, mask)
+    if mask is not None:
+        mask = (mask if mask.dtype == torch.bool else mask != 0).view(torch.uint8)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, h0)):
+        return _GatedScan.apply(x, gate, h0, mask)
+    y, hT, _ = _forward(_dense(x), _dense(gate), None if h0 is None else h0.contiguous(), mask, False)
+    return y, hT

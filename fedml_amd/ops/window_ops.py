@@ -1,0 +1,404 @@
+"""Causal sliding-window attention with sinks and a bucketed relative position bias, for long text
+(``csrc/window_kernels.hip``).
+
+* :func:`window_attention` — forward and backward over whole sequences of any length: token i sees the ``window`` last
+  tokens up to itself and the first ``sinks`` tokens; ``kv_heads`` ≤ H shared key/value heads; a token mask; a learned
+  bias per head and distance bucket (``bias``), with its gradient.
+* :func:`window_attention_step` — the same for ONE new token per sequence over a ring cache of ``sinks + window``
+  slots, which it updates; :func:`window_cache_fill` puts a prompt's keys and values there.
+* :func:`relative_bucket_starts` — the first distance of every bucket.
+
+Rows are token-major ``[sequences · S, heads · D]``, head h at columns ``[h·D, (h+1)·D)``, D = 64 or 128, bf16 or fp32
+(row strides may exceed heads · D: column slices of a fused projection are read in place). CUDA tensors run the HIP
+kernels at the storage precision with fp32 sums and statistics; CPU tensors run the plain-PyTorch form of the same
+mathematics (fp64 for fp64 inputs), which is also the tests' oracle. All results are the same bit for bit from call to
+call: no atomics. Everything is enqueued on the current stream of the tensors' device and may be captured into a HIP
+graph; scratch memory is allocated per call."""
+import ctypes as _c
+import functools
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .fl_ops import _check, _fn, _i64, _p, _pr, _stream, use_native
+
+MAX_SINKS = 64
+MAX_BUCKETS = 128
+MAX_DISTANCE = 1024
+_I32 = 2 ** 31 - 1
+
+
+class _Args(_c.Structure):
+    _fields_ = [(n, _c.c_void_p) for n in ("q", "k", "v", "dout", "o", "olo", "dq", "dk", "dv", "lse", "dsum", "part",
+                                           "bpart", "dbias", "mask", "bias")] + \
+               [(n, _c.c_int64) for n in ("ldq", "ldk", "ldv", "lddo")] + \
+               [(n, _c.c_int) for n in ("N", "S", "H", "KV", "C", "W", "sinks", "NB", "maxd", "nchunk", "qchunk")] + \
+               [("scale", _c.c_float), ("start", _c.c_int * MAX_BUCKETS)]
+
+
+class _StepArgs(_c.Structure):
+    _fields_ = [(n, _c.c_void_p) for n in ("q", "k", "v", "kc", "vc", "o", "pos", "bias", "pacc", "pml")] + \
+               [(n, _c.c_int64) for n in ("ldq", "ldk", "ldv")] + \
+               [(n, _c.c_int) for n in ("B", "H", "KV", "C", "W", "sinks", "NB", "maxd", "splits", "per")] + \
+               [("scale", _c.c_float), ("start", _c.c_int * MAX_BUCKETS)]
+
+
+@functools.lru_cache(maxsize=None)
+def relative_bucket_starts(buckets: int, max_distance: int):
+    """First distance of every bucket: one distance each below E = buckets // 2, then evenly over the logarithm up to
+    ``max_distance``; the last bucket has no end. bucket(d) = d for d < E, else
+    min(buckets − 1, E + ⌊n·log(d/E) / log(max_distance/E)⌋) with n = buckets − E, decided in whole numbers
+    (d^n ≥ max_distance^j · E^(n−j)), so that no rounding moves a border."""
+    buckets, M = int(buckets), int(max_distance)
+    if not 2 <= buckets <= MAX_BUCKETS:
+        raise ValueError(f"relative bias: 2 to {MAX_BUCKETS} buckets, got {buckets}")
+    E = buckets // 2
+    n = buckets - E
+    if not E < M <= MAX_DISTANCE:
+        raise ValueError(f"relative bias: max_distance in ({E}, {MAX_DISTANCE}] for {buckets} buckets, got {M}")
+    starts, d = list(range(E + 1)), E
+    for j in range(1, n):
+        while d ** n < M ** j * E ** (n - j):
+            d += 1
+        starts.append(d)
+    return tuple(starts)
+
+
+def relative_bucket(distance: torch.Tensor, buckets: int, max_distance: int) -> torch.Tensor:
+    """Bucket of every (whole, ≥ 0) distance."""
+    starts = torch.tensor(relative_bucket_starts(buckets, max_distance), device=distance.device)
+    return torch.bucketize(distance, starts, right=True) - 1
+
+
+# ------------------------------------------------------------------------------------------------- argument checks
+def _rows(t, heads, name, rows=None, dtype=None, device=None):
+    """(D, rows) of a token-major operand."""
+    if t.dim() != 2 or heads < 1 or t.shape[1] % heads:
+        raise ValueError(f"{name}: [rows, heads · D] with {heads} heads expected, got {tuple(t.shape)}")
+    if t.dtype not in (torch.bfloat16, torch.float32) and (t.is_cuda or t.dtype != torch.float64):
+        raise TypeError(f"{name}: bf16 or fp32 expected, got {t.dtype}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name}: {dtype} expected, got {t.dtype}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, q on {device}")
+    if rows is not None and t.shape[0] != rows:
+        raise ValueError(f"{name}: {rows} rows expected, got {t.shape[0]}")
+    return t.shape[1] // heads
+
+
+def _common(q, k, v, H, kv_heads, window, sinks):
+    H, KV = int(H), int(H if kv_heads is None else kv_heads)
+    if H < 1 or KV < 1 or H % KV:
+        raise ValueError(f"H = {H} query heads over {KV} key/value heads")
+    D = _rows(q, H, "q")
+    if D not in (64, 128):
+        raise ValueError(f"head dim 64 or 128 expected, got {D}")
+    for t, n in ((k, "k"), (v, "v")):
+        if _rows(t, KV, n, q.shape[0], q.dtype, q.device) != D:
+            raise ValueError(f"{n}: {KV} heads of dim {D} expected, got {tuple(t.shape)}")
+    if not 1 <= int(window) <= _I32:
+        raise ValueError(f"window ≥ 1 expected, got {window}")
+    if not 0 <= int(sinks) <= MAX_SINKS:
+        raise ValueError(f"sinks in [0, {MAX_SINKS}] expected, got {sinks}")
+    return D, H, KV, int(window), int(sinks)
+
+
+def _bias(bias, sequences, H, max_distance, device):
+    """The table as [C, H, buckets] and its borders."""
+    if bias is None:
+        return None, ()
+    if bias.dim() not in (2, 3) or bias.shape[-2] != H:
+        raise ValueError(f"bias: [H, buckets] or [C, H, buckets] with H = {H} expected, got {tuple(bias.shape)}")
+    if bias.device != device:
+        raise ValueError(f"bias is on {bias.device}, q on {device}")
+    if bias.dtype != torch.float32 and (bias.is_cuda or bias.dtype != torch.float64):
+        raise TypeError(f"bias: fp32 expected, got {bias.dtype}")
+    if bias.dim() == 2:
+        bias = bias.unsqueeze(0)
+    C = bias.shape[0]
+    if C < 1 or sequences % C:
+        raise ValueError(f"bias of {C} clients for {sequences} sequences")
+    return bias, relative_bucket_starts(bias.shape[-1], max_distance)
+
+
+def _scale(scale, D):
+    return 1.0 / math.sqrt(D) if scale is None else float(scale)
+
+
+def _aligned(t):
+    """16-byte rows for the kernels: the tensor itself where its rows are, else a dense copy."""
+    e = 16 // t.element_size()
+    if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) % e == 0 and t.stride(0) >= t.shape[1] and \
+            t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _v(p):
+    return None if p is None else p.value
+
+
+def _launch(name, args, dtype, D, t):
+    bf16 = int(dtype == torch.bfloat16)
+    with torch.cuda.device(t.device):
+        _check(_fn(name)(_c.byref(args), _c.c_int(bf16), _c.c_int(D), _stream(t)), name)
+
+
+# ------------------------------------------------------------------------------------------------------- reference
+def _ct(t):
+    return torch.float64 if t.dtype == torch.float64 else torch.float32
+
+
+def _bias_of(bias, distance, sequences, max_distance, ct):
+    """[sequences, H, ·] bias of whole distances (negative ones: any value)."""
+    b = relative_bucket(distance.clamp_min(0), bias.shape[-1], max_distance)
+    return bias.to(ct)[..., b].repeat_interleave(sequences // bias.shape[0], 0)
+
+
+def _window_ref(q, k, v, S, H, KV, W, sinks, mask, bias, max_distance, scale):
+    N, D, ct = q.shape[0] // S, q.shape[1] // H, _ct(q)
+    real = torch.ones(N, S, dtype=torch.bool, device=q.device) if mask is None else mask.bool()
+
+    def heads(t, h):     # what is no token is zero, whatever it holds
+        return torch.where(real.view(N, S, 1, 1), t.to(ct).view(N, S, h, D), torch.zeros((), dtype=ct, device=q.device)
+                           ).transpose(1, 2)
+
+    qh, kh, vh = heads(q, H), *(heads(t, KV).repeat_interleave(H // KV, 1) for t in (k, v))
+    i = torch.arange(S, device=q.device)
+    d = i.view(S, 1) - i
+    see = (d >= 0) & ((d < W) | (i < sinks))
+    see = (see & real.view(N, 1, S) & real.view(N, S, 1)).unsqueeze(1)
+    s = qh @ kh.transpose(-1, -2) * scale
+    if bias is not None:
+        s = s + _bias_of(bias, d, N, max_distance, ct)
+    s = s.masked_fill(~see, float("-inf"))
+    p = torch.softmax(s.masked_fill(~see.any(-1, keepdim=True), 0.0), -1)
+    p = torch.where(see, p, torch.zeros((), dtype=ct, device=q.device))
+    o = torch.where(real.view(N, 1, S, 1), p @ vh, torch.zeros((), dtype=ct, device=q.device))
+    return o.transpose(1, 2).reshape(N * S, H * D).to(q.dtype)
+
+
+# --------------------------------------------------------------------------------------------------------- training
+def _args(q, k, v, mask, bias, starts, cfg):
+    S, H, KV, W, sinks, D, max_distance, scale = cfg
+    a = _Args(q=_v(_pr(q)), k=_v(_pr(k)), v=_v(_pr(v)), mask=_v(_pr(mask)), bias=_v(_pr(bias)), ldq=q.stride(0),
+              ldk=k.stride(0), ldv=v.stride(0), N=q.shape[0] // S, S=S, H=H, KV=KV, C=1 if bias is None else
+              bias.shape[0], W=W, sinks=sinks, NB=len(starts), maxd=max_distance if starts else 0, scale=scale)
+    a.start[:len(starts)] = starts
+    return a
+
+
+def _forward(q, k, v, mask, bias, starts, cfg, keep, exact):
+    """(o, what its rounding left over, log-sum-exp); keep: for a backward pass, exact: with a gradient of the bias."""
+    S, H, D = cfg[0], cfg[1], cfg[5]
+    o = torch.empty(q.shape[0], H * D, dtype=q.dtype, device=q.device)
+    olo = torch.empty_like(o) if exact and q.dtype == torch.bfloat16 else None
+    lse = torch.empty(q.shape[0] // S, H, S, dtype=torch.float32, device=q.device) if keep else None
+    if q.shape[0]:
+        a = _args(q, k, v, mask, bias, starts, cfg)
+        a.o, a.olo, a.lse = _v(_p(o)), _v(_p(olo)), _v(_p(lse))
+        _launch("fa_window_fwd", a, q.dtype, D, q)
+    return o, olo, lse
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, bias, mask, starts, cfg):
+        q, k, v = _aligned(q), _aligned(k), _aligned(v)
+        tab = None if bias is None else bias.contiguous()
+        o, olo, lse = _forward(q, k, v, mask, tab, starts, cfg, True, bias is not None and ctx.needs_input_grad[3])
+        ctx.save_for_backward(q, k, v, tab, mask, o, olo, lse)
+        ctx.starts, ctx.cfg = starts, cfg
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, bias, mask, o, olo, lse = ctx.saved_tensors
+        S, H, KV, W, sinks, D, _, _ = ctx.cfg
+        N, dev = q.shape[0] // S, q.device
+        do = _aligned(do.to(q.dtype))
+        dq = torch.empty(N * S, H * D, dtype=q.dtype, device=dev)
+        dk = torch.empty(N * S, KV * D, dtype=q.dtype, device=dev)
+        dv = torch.empty_like(dk)
+        dbias = torch.zeros_like(bias) if bias is not None and ctx.needs_input_grad[3] else None
+        if N:
+            a = _args(q, k, v, mask, bias, ctx.starts, ctx.cfg)
+            tile = 128 if S > 64 else 32                  # queries of a workgroup of the dq kernel
+            dsum = torch.empty(N, H, S, dtype=torch.float32, device=dev)
+            part = bpart = None
+            if sinks and S > W:
+                a.qchunk = max(512, -(-(W + 128) // 128) * 128)
+                a.nchunk = -(-(S - W) // a.qchunk)
+                part = torch.empty(N, KV, a.nchunk + 1, 2, sinks, D, dtype=torch.float32, device=dev)
+            if dbias is not None:
+                bpart = torch.empty(N, H, -(-S // tile), bias.shape[-1], dtype=torch.float32, device=dev)
+            a.dout, a.lddo, a.lse, a.o, a.olo = _v(_pr(do)), do.stride(0), _v(_pr(lse)), _v(_pr(o)), _v(_pr(olo))
+            a.dq, a.dk, a.dv, a.dsum = _v(_p(dq)), _v(_p(dk)), _v(_p(dv)), _v(_p(dsum))
+            a.part, a.bpart, a.dbias = _v(_p(part)), _v(_p(bpart)), _v(_p(dbias))
+            _launch("fa_window_bwd", a, q.dtype, D, q)
+        return dq, dk, dv, dbias, None, None, None
+
+
+def window_attention(q, k, v, S: int, H: int, window: int, sinks: int = 0, kv_heads: int = None,
+                     mask: torch.Tensor = None, bias: torch.Tensor = None, max_distance: int = 128,
+                     scale: float = None):
+    """Causal attention of ``q`` [N·S, H·D] over ``k`` / ``v`` [N·S, kv_heads·D], N sequences of S tokens: token i sees
+    token j ≤ i if i − j < ``window`` or j < ``sinks`` (≤ 64). Query head h reads key/value head h // (H / kv_heads).
+
+    ``mask`` [N, S] (bool or integer, nonzero = a token): what is no token is neither a key nor a query — its output row
+    is zero, its gradients are zero, and what its rows hold (NaN included) reaches nothing. Distances and sinks count
+    positions, so pad on the right. ``bias`` [H, buckets] or per-client [C, H, buckets] (fp32; sequences [c·N/C,
+    (c+1)·N/C) are client c's) is added to the scaled scores by :func:`relative_bucket_starts`' bucket of i − j.
+    ``scale``: 1/√D unless given. Gradients: q, k, v (at their type) and bias (fp32).
+
+    A non-finite value in a real token's rows reaches every row that sees the token, and may reach others near it."""
+    D, H, KV, W, sinks = _common(q, k, v, H, kv_heads, window, sinks)
+    S = int(S)
+    if S < 1 or q.shape[0] % S:
+        raise ValueError(f"{q.shape[0]} rows are no whole sequences of {S} tokens")
+    N = q.shape[0] // S
+    if N * S > _I32 or N * H * S > _I32:
+        raise ValueError(f"{N} sequences · {H} heads · {S} tokens: at most 2^31 − 1")
+    if mask is not None:
+        if mask.shape != (N, S) or mask.dtype.is_floating_point or mask.dtype.is_complex or mask.device != q.device:
+            raise ValueError(f"mask: bool or integer [{N}, {S}] on {q.device} expected, got {mask.dtype} "
+                             f"{tuple(mask.shape)} on {mask.device}")
+    table, starts = _bias(bias, N, H, max_distance, q.device)
+    scale = _scale(scale, D)
+    if not use_native(q):
+        return _window_ref(q, k, v, S, H, KV, W, sinks, mask, table, max_distance, scale)
+    if mask is not None:
+        mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous().view(torch.uint8)
+    cfg = (S, H, KV, min(W, S), min(sinks, S), D, int(max_distance), scale)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table)):
+        return _WindowAttention.apply(q, k, v, table, mask, starts, cfg)
+    tab = None if table is None else table.contiguous()
+    return _forward(_aligned(q), _aligned(k), _aligned(v), mask, tab, starts, cfg, False, False)[0]
+
+
+# ---------------------------------------------------------------------------------------------------------- serving
+def _cache(k_cache, v_cache, B, KV, D, slots, dtype, device):
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if tuple(t.shape) != (B, slots, KV * D) or t.dtype != dtype or t.device != device:
+            raise ValueError(f"{n}: {dtype} [{B}, {slots}, {KV * D}] on {device} expected, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+        if not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f"{n}: contiguous, 16-byte aligned memory expected (it is updated in place)")
+        if t.requires_grad:
+            raise ValueError(f"{n} takes no gradient")
+
+
+def _pos(pos, B, device, name):
+    if pos.shape != (B,) or pos.dtype != torch.int32 or pos.device != device:
+        raise ValueError(f"{name}: int32 [{B}] on {device} expected, got {pos.dtype} {tuple(pos.shape)} on {pos.device}")
+    return pos.contiguous()
+
+
+def _slot_tokens(pos, slots, window, sinks):
+    """The token in every slot once token ``pos`` [B] is there, −1 where there is none: [B, slots]."""
+    pos = pos.long().view(-1, 1)
+    s = torch.arange(slots, device=pos.device).view(1, -1)
+    ring = pos - (pos - s) % window
+    ring = torch.where((pos >= sinks) & (ring >= sinks), ring, -1)
+    return torch.where(s < sinks, torch.where(s <= pos, s, -1), ring)
+
+
+def _step_ref(q, k, v, kc, vc, pos, H, KV, W, sinks, bias, max_distance, scale):
+    B, n, D, ct = q.shape[0], kc.shape[1], q.shape[1] // H, _ct(q)
+    tok = _slot_tokens(pos, n, W, sinks)
+    p = pos.long().view(-1, 1)
+    here = (tok == p) & (p >= 0)
+    kc.copy_(torch.where(here.unsqueeze(-1), k.unsqueeze(1), kc))
+    vc.copy_(torch.where(here.unsqueeze(-1), v.unsqueeze(1), vc))
+    see = (tok >= 0) & (p >= 0)
+    zero = torch.zeros((), dtype=ct, device=q.device)
+    kh, vh = (torch.where(see.view(B, n, 1, 1), t.to(ct).view(B, n, KV, D), zero).transpose(1, 2)
+              .repeat_interleave(H // KV, 1) for t in (kc, vc))
+    s = (q.to(ct).view(B, H, 1, D) @ kh.transpose(-1, -2)).squeeze(2) * scale
+    if bias is not None:
+        b = relative_bucket((p - tok).clamp_min(0), bias.shape[-1], max_distance)                     # [B, n]
+        tab = bias.to(ct).repeat_interleave(B // bias.shape[0], 0)
+        s = s + tab.gather(2, b.unsqueeze(1).expand(B, H, n))
+    s = s.masked_fill(~see.unsqueeze(1), float("-inf")).masked_fill(~see.any(1).view(B, 1, 1), 0.0)
+    w = torch.where(see.unsqueeze(1), torch.softmax(s, -1), zero)
+    return (w.unsqueeze(2) @ vh).reshape(B, H * D).to(q.dtype)
+
+
+def window_attention_step(q, k, v, k_cache, v_cache, pos, H: int, window: int, sinks: int = 0, kv_heads: int = None,
+                          bias: torch.Tensor = None, max_distance: int = 128, scale: float = None):
+    """:func:`window_attention` of one new token per sequence: ``q`` [B, H·D], ``k`` / ``v`` [B, kv_heads·D] are its
+    rows, ``pos`` int32 [B] its position (the number of tokens before it). ``k_cache`` / ``v_cache`` [B, sinks + window,
+    kv_heads·D] hold token t < sinks in slot t and token t in slot sinks + (t − sinks) % window: the new token's rows are
+    written there (over the token that leaves the window) and the output [B, H·D] is returned. A sequence with
+    ``pos`` < 0 is idle: its cache stays as it is and its output is zero. Slots that hold no token yet are not read. The
+    caller counts ``pos`` on, once per token for all layers; no gradient."""
+    D, H, KV, W, sinks = _common(q, k, v, H, kv_heads, window, sinks)
+    B, n = q.shape[0], W + sinks
+    _cache(k_cache, v_cache, B, KV, D, n, q.dtype, q.device)
+    pos = _pos(pos, B, q.device, "pos")
+    table, starts = _bias(bias, B, H, max_distance, q.device)
+    scale = _scale(scale, D)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
+        raise ValueError("window_attention_step computes no gradient: call it under torch.no_grad()")
+    if not use_native(q):
+        return _step_ref(q, k, v, k_cache, v_cache, pos, H, KV, W, sinks, table, max_distance, scale)
+    o = torch.empty(B, H * D, dtype=q.dtype, device=q.device)
+    if B == 0:
+        return o
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    tab = None if table is None else table.contiguous()
+    # enough workgroups for 256 CUs, of at least one 32-slot tile a wave
+    wgs = B * KV * -(-(H // KV) // 32)
+    tiles = -(-n // 128)
+    splits = max(1, min(tiles, -(-512 // wgs)))
+    per = -(-tiles // splits) * 128
+    splits = -(-n // per)
+    if wgs * splits > _I32 or B * H > _I32:
+        raise ValueError(f"{B} sequences of {H} heads are too many for one call")
+    a = _StepArgs(q=_v(_pr(q)), k=_v(_pr(k)), v=_v(_pr(v)), kc=_v(_p(k_cache)), vc=_v(_p(v_cache)), o=_v(_p(o)),
+                  pos=_v(_pr(pos)), bias=_v(_pr(tab)), ldq=q.stride(0), ldk=k.stride(0), ldv=v.stride(0), B=B, H=H,
+                  KV=KV, C=1 if tab is None else tab.shape[0], W=W, sinks=sinks, NB=len(starts),
+                  maxd=int(max_distance) if starts else 0, splits=splits, per=per, scale=scale)
+    a.start[:len(starts)] = starts
+    if splits > 1:
+        part = torch.empty(B * H * splits * (D + 2), dtype=torch.float32, device=q.device)
+        a.pacc, a.pml = _v(_p(part)), _v(_p(part[B * H * splits * D:]))
+    _launch("fa_window_step", a, q.dtype, D, q)
+    return o
+
+
+def window_cache_fill(k, v, S: int, k_cache, v_cache, window: int, sinks: int = 0, lengths: torch.Tensor = None):
+    """Puts a prompt's rows ``k`` / ``v`` [B·S, kv_heads·D] into the caches of :func:`window_attention_step`, as its
+    steps would have left them after token ``lengths[b]`` − 1 (int32 [B], within [0, S]; all S tokens if not given).
+    Slots that hold none of these tokens stay as they were."""
+    if k_cache.dim() != 3:
+        raise ValueError(f"k_cache: [B, sinks + window, kv_heads · D] expected, got {tuple(k_cache.shape)}")
+    B, S, W, sinks, width = k_cache.shape[0], int(S), int(window), int(sinks), k_cache.shape[2]
+    if not 1 <= W <= _I32 or not 0 <= sinks <= MAX_SINKS or S < 1:
+        raise ValueError(f"window ≥ 1, sinks in [0, {MAX_SINKS}] and S ≥ 1 expected, got {window}, {sinks}, {S}")
+    for t, n in ((k, "k"), (v, "v")):
+        _rows(t, 1, n, B * S, k_cache.dtype, k_cache.device)
+        if t.shape[1] != width or width % 64:
+            raise ValueError(f"{n}: rows of the cache's {width} columns expected, got {t.shape[1]}")
+    _cache(k_cache, v_cache, B, 1, width, W + sinks, k.dtype, k.device)
+    if lengths is not None:
+        lengths = _pos(lengths, B, k.device, "lengths")
+    with torch.no_grad():
+        if not use_native(k):
+            last = (torch.full((B,), S, device=k.device) if lengths is None else lengths.clamp(0, S)) - 1
+            tok = _slot_tokens(last, W + sinks, W, sinks)
+            at = tok.clamp_min(0) + torch.arange(B, device=k.device).view(B, 1) * S
+            for t, c in ((k, k_cache), (v, v_cache)):
+                c.copy_(torch.where((tok >= 0).unsqueeze(-1), t[at], c))
+            return
+        if B == 0:
+            return
+        k, v = _aligned(k), _aligned(v)
+        e = 16 // k.element_size()
+        with torch.cuda.device(k.device):
+            rc = _fn("fa_window_fill")(_pr(k), _pr(v), _i64(k.stride(0) // e), _i64(v.stride(0) // e), _p(k_cache),
+                                       _p(v_cache), _pr(lengths), _c.c_int(B), _c.c_int(S), _c.c_int(W),
+                                       _c.c_int(sinks), _c.c_int(width // e), _stream(k))
+            _check(rc, "fa_window_fill")

@@ -1,0 +1,89 @@
+"""Gated linear recurrence on the CPU path: the plain form against the definition step by step, gradients against
+differences, pieces against the whole, padding, refusals."""
+import math
+
+import pytest
+import torch
+
+from fedml_amd import ops
+
+
+def _inputs(C, T, B, H, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(C, T, B, H, generator=gen, dtype=torch.float64),
+            torch.randn(C, T, B, H, generator=gen, dtype=torch.float64) * 3,
+            torch.randn(C, B, H, generator=gen, dtype=torch.float64))
+
+
+def test_reference_is_the_definition():
+    x, gate, h0 = _inputs(2, 5, 2, 3)
+    mask = torch.tensor([[[1, 1], [1, 0], [0, 1], [1, 1], [0, 1]], [[1, 1]] * 5])
+    y, hT = ops.gated_scan(x, gate, h0, mask=mask)
+    for c in range(2):
+        for b in range(2):
+            for j in range(3):
+                h = float(h0[c, b, j])
+                for t in range(5):
+                    if mask[c, t, b]:
+                        f = 1 / (1 + math.exp(-float(gate[c, t, b, j])))
+                        h = f * h + (1 - f) * float(x[c, t, b, j])
+                        assert abs(float(y[c, t, b, j]) - h) < 1e-14
+                    else:
+                        assert float(y[c, t, b, j]) == 0.0
+                assert abs(float(hT[c, b, j]) - h) < 1e-14
+
+
+def test_gradients_are_differences():
+    x, gate, h0 = (t.requires_grad_() for t in _inputs(1, 6, 2, 3, 1))
+    mask = torch.ones(1, 6, 2, dtype=torch.bool)
+    mask[0, 4:, 1] = False
+    assert torch.autograd.gradcheck(lambda *a: ops.gated_scan(*a, mask=mask), (x, gate, h0))
+
+
+def test_pieces_are_the_whole():
+    x, gate, h0 = _inputs(1, 9, 2, 4, 2)
+    y, hT = ops.gated_scan(x, gate, h0)
+    h, ys = h0, []
+    for part in (slice(0, 1), slice(1, 6), slice(6, 9)):
+        z, h = ops.gated_scan(x[:, part], gate[:, part], h)
+        ys.append(z)
+    assert torch.equal(torch.cat(ys, 1), y) and torch.equal(h, hT)
+    z, _ = ops.gated_scan(x, gate)
+    assert torch.equal(z, ops.gated_scan(x, gate, torch.zeros_like(h0))[0])
+
+
+def test_padding_reaches_nothing():
+    x, gate, h0 = _inputs(1, 5, 2, 3, 3)
+    mask = torch.ones(1, 5, 2, dtype=torch.bool)
+    mask[0, 2:, 0] = False
+    mask[0, :, 1] = False
+    bad = [t.clone() for t in (x, gate)]
+    for t in bad:
+        t[~mask] = float("nan")
+        t.requires_grad_()
+    y, hT = ops.gated_scan(*bad, h0, mask=mask)
+    ref, h = ops.gated_scan(x[:, :2, :1], gate[:, :2, :1], h0[:, :1])
+    assert torch.equal(y[:, :2, :1], ref) and torch.equal(hT[:, :1], h) and torch.equal(hT[:, 1], h0[:, 1])
+    assert not y[~mask].any()
+    gy = torch.ones_like(y)
+    gy[~mask] = float("nan")
+    for g in torch.autograd.grad((y, hT), bad, (gy, torch.ones_like(hT))):
+        assert torch.isfinite(g).all() and not g[~mask].any()
+
+
+def _t(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("error,match,kw", [
+    (ValueError, "expected", dict(x=_t(2, 3, 4))), (ValueError, "expected", dict(gate=_t(1, 3, 2, 5))),
+    (TypeError, "bf16 or fp32", dict(x=_t(1, 3, 2, 4, dtype=torch.float16), gate=_t(1, 3, 2, 4, dtype=torch.float16))),
+    (TypeError, "gate", dict(gate=_t(1, 3, 2, 4, dtype=torch.bfloat16))),
+    (ValueError, "at least one", dict(x=_t(1, 0, 2, 4), gate=_t(1, 0, 2, 4))),
+    (ValueError, "h0", dict(h0=_t(1, 2, 5))), (ValueError, "h0", dict(h0=_t(1, 2, 4, dtype=torch.bfloat16))),
+    (ValueError, "mask", dict(mask=_t(1, 3, 2))), (ValueError, "mask", dict(mask=torch.ones(1, 2, 3, dtype=torch.bool)))])
+def test_refusals(error, match, kw):
+    a = dict(x=_t(1, 3, 2, 4), gate=_t(1, 3, 2, 4))
+    a.update(kw)
+    with pytest.raises(error, match=match):
+        ops.gated_scan(**a)

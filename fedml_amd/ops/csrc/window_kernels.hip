@@ -27,19 +27,21 @@ typedef short v4i16 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kGrow = 8.f;      // see fwd_kernel
 constexpr int kMaxBuckets = 128;
 constexpr int kLutOff = 62;      // a processed 32×32 block holds distances >= −62 (the negative ones are masked)
 constexpr int kBinPad = 64;      // distances of a block that starts below max_distance end below max_distance + 62
 
 struct Args {
   const void *q, *k, *v, *dout;
-  void *o, *olo, *dq, *dk, *dv;
-  float *lse, *dsum, *part, *bpart, *dbias;
+  void *o, *dq, *dk, *dv;
+  float *o32, *lse, *dsum, *part, *bpart, *dbias;
   const uint8_t* mask;
   const float* bias;
   int64_t ldq, ldk, ldv, lddo;
   int N, S, H, KV, C, W, sinks, NB, maxd;
   int nchunk, qchunk;            // sink pass of the backward: chunks of queries
+  int exact;                     // forward: a gradient of the bias follows
   float scale;
   int start[kMaxBuckets];        // first distance of every bucket
 };
@@ -60,22 +62,25 @@ template <> struct Elem<uint16_t> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                    0, 0);
   }
-  static __device__ __forceinline__ float dot(uint4 a, uint4 b, float s) {
-    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+  // a unit times as many fp32 values
+  static __device__ __forceinline__ float dot(uint4 a, const float* y, float s) {
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      s = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), s);
-      s = fmaf(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), s);
+      const float2 b = *reinterpret_cast<const float2*>(y + 2 * i);
+      s = fmaf(__uint_as_float(x[i] << 16), b.x, s);
+      s = fmaf(__uint_as_float(x[i] & 0xffff0000u), b.y, s);
     }
     return s;
   }
-  // four consecutive columns; lo (optional): what the rounding left over
+  // four consecutive columns
   static __device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, float d) {
     uint2 u;
     u.x = (uint32_t)f32_to_bf16(a) | ((uint32_t)f32_to_bf16(b) << 16);
     u.y = (uint32_t)f32_to_bf16(c) | ((uint32_t)f32_to_bf16(d) << 16);
     *reinterpret_cast<uint2*>(p) = u;
   }
+  // what the rounding of a leaves over
   static __device__ __forceinline__ float left(float a) { return a - bf16_to_f32(f32_to_bf16(a)); }
 };
 template <> struct Elem<float> {
@@ -87,9 +92,9 @@ template <> struct Elem<float> {
     c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, y.z, c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, y.w, c, 0, 0, 0);
   }
-  static __device__ __forceinline__ float dot(uint4 a, uint4 b, float s) {
-    const float4 x = __builtin_bit_cast(float4, a), y = __builtin_bit_cast(float4, b);
-    return fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s))));
+  static __device__ __forceinline__ float dot(uint4 a, const float* y, float s) {
+    const float4 x = __builtin_bit_cast(float4, a), b = *reinterpret_cast<const float4*>(y);
+    return fmaf(x.x, b.x, fmaf(x.y, b.y, fmaf(x.z, b.z, fmaf(x.w, b.w, s))));
   }
   static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
     *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
@@ -102,6 +107,29 @@ __device__ __forceinline__ f32x16 zero16() {
 #pragma unroll
   for (int r = 0; r < 16; ++r) z[r] = 0.f;
   return z;
+}
+
+// over the two halves of the wave (which hold the same column)
+__device__ __forceinline__ float half_max(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+
+// What a 32×32 block of scores (queries from q, keys from k) is to a wave: seen at all, seen whole
+__device__ __forceinline__ bool block_seen(const Args& a, int q, int k) {
+  return q < a.S && k < a.S && k <= q + 31 && (q - k - 31 < a.W || k < a.sinks);
+}
+__device__ __forceinline__ bool block_whole(const Args& a, int q, int k) {
+  return k + 31 <= q && (q + 31 - k < a.W || k + 31 < a.sinks);
+}
+// bit j: key k0 + j is a token, for the 32 keys of a block
+__device__ __forceinline__ uint32_t token_bits(const Args& a, const uint8_t* mask, int k0, int lane) {
+  const int key = k0 + (lane & 31);
+  return (uint32_t)__ballot(key < a.S && (!mask || mask[key]));
 }
 
 // A head's rows and how they lie in registers and LDS
@@ -218,10 +246,10 @@ struct KeyTiles {
 // of BK with a running maximum and sum. The next tile's rows are in flight in registers during a tile's products.
 // Probabilities are rounded to the storage type for the product with v (half a step each, 2^-8 in bf16, and the sum is
 // of the unrounded ones). EXACT (bf16, before a gradient of the bias): what that rounding leaves over goes through a
-// second product and what the output's leaves over is kept, so that D = dO·o is good to 2^-16 — dbias is fp32.
+// second product, so that D = dO·o of the unrounded output is good to 2^-16 — dbias is fp32.
 // ----------------------------------------------------------------------------------------------------------------
-template <typename T, int D, int NW, int BK, bool EXACT>
-__global__ __launch_bounds__(64 * NW) void fwd_kernel(const Args a) {
+template <typename T, int D, int NW, int BK, bool BIAS, bool EXACT>
+__global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void fwd_kernel(const Args a) {
   using R = Row<T, D>;
   __shared__ __attribute__((aligned(16))) T Ks[BK * R::P];
   __shared__ __attribute__((aligned(16))) T Vs[BK * R::P];
@@ -242,7 +270,7 @@ __global__ __launch_bounds__(64 * NW) void fwd_kernel(const Args a) {
   const bool real = qi < a.S && (!mask || mask[qi]);
   uint4 qf[R::NC];
   R::frags(qf, (const T*)a.q + (tok0 + qi) * a.ldq + h * D, real, hh);
-  if (a.bias) fill_lut(lut, a, n / (a.N / a.C), h, tid, 64 * NW);
+  if (BIAS) fill_lut(lut, a, n / (a.N / a.C), h, tid, 64 * NW);
   const KeyTiles tiles(a, q0, 32 * NW, BK);
   const int count = __syncthreads_or(real) ? tiles.count : 0;
   const float c2 = a.scale * kLog2e;
@@ -265,66 +293,76 @@ __global__ __launch_bounds__(64 * NW) void fwd_kernel(const Args a) {
       sk.load(kp, a.ldk, tiles.at(it + 1) * BK, a.S, mask, tid);
       sv.load(vp, a.ldv, tiles.at(it + 1) * BK, a.S, mask, tid);
     }
+    constexpr int NB = BK / 32;
+    f32x16 s[NB];
+    bool seen[NB], any = false;
+    float mt = -INFINITY;
 #pragma unroll
-    for (int sub = 0; sub < BK / 32; ++sub) {
-      const int kb = k0 + 32 * sub;
-      if (qw >= a.S || kb >= a.S || kb > qw + 31 || !(qw - kb - 31 < a.W || kb < a.sinks)) continue;
-      f32x16 s = R::rows(Ks + 32 * sub * R::P, qf, lane);
-      const uint32_t bits =
-          (uint32_t)__ballot(kb + (lane & 31) < a.S && (!mask || mask[kb + (lane & 31)])) >> (4 * hh);
-      const bool all = !__any(bits != (hh ? 0x0fffffffu : 0xffffffffu)) && kb + 31 <= qw &&
-                       (qw + 31 - kb < a.W || kb + 31 < a.sinks);
-      if (a.bias) {
+    for (int b = 0; b < NB; ++b) {
+      const int kb = k0 + 32 * b;
+      seen[b] = block_seen(a, qw, kb);
+      if (!seen[b]) continue;
+      any = true;
+      s[b] = R::rows(Ks + 32 * b * R::P, qf, lane);
+      const uint32_t bits = token_bits(a, mask, kb, lane);
+      if (BIAS) {
         if (qw - kb - 31 < a.maxd) {
           const float* at = lut + kLutOff + qi - kb - 4 * hh;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, at[-kappa(r)]);
+          for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], c2, at[-kappa(r)]);
         } else {
           const float far = lut[lut_size(a.maxd) - 1];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, far);
+          for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], c2, far);
         }
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= c2;
       }
-      if (!all) {
+      if (bits != 0xffffffffu || !block_whole(a, qw, kb)) {
+        const uint32_t mine = bits >> (4 * hh);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int key = kb + kappa(r) + 4 * hh;
-          const bool see = key <= qi && (qi - key < a.W || key < a.sinks) && ((bits >> kappa(r)) & 1);
-          s[r] = see ? s[r] : -INFINITY;
+          const bool see = key <= qi && (qi - key < a.W || key < a.sinks) && ((mine >> kappa(r)) & 1);
+          s[b][r] = see ? s[b][r] : -INFINITY;
         }
       }
-      float mt = s[0];
 #pragma unroll
-      for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
-      mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-      const float mn = fmaxf(m, mt), mu = mn == -INFINITY ? 0.f : mn;
-      if (__any(mn > m)) {
-        const float al = __builtin_amdgcn_exp2f(m - mu);
-        l *= al;
+      for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[b][r]);
+    }
+    if (!any) continue;
+    mt = half_max(mt);
+    if (!BIAS) mt *= c2;
+    if (__any(mt > m + kGrow)) {
+      const float mn = fmaxf(m, mt), al = __builtin_amdgcn_exp2f(m - mn);   // m = −inf: 0 (mn is finite or the row is NaN)
+      const float x = mn == -INFINITY ? 1.f : al;
+      l *= x;
 #pragma unroll
-        for (int db = 0; db < R::DB; ++db)
+      for (int db = 0; db < R::DB; ++db)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[db][r] *= al;
-      }
+        for (int r = 0; r < 16; ++r) acc[db][r] *= x;
       m = mn;
+    }
+    const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      if (!seen[b]) continue;
       float p[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        p[r] = __builtin_amdgcn_exp2f(s[r] - mu);
+        p[r] = __builtin_amdgcn_exp2f(BIAS ? s[b][r] - mu : fmaf(s[b][r], c2, -mu));
         l += p[r];
       }
-      R::cols(acc, Vs + 32 * sub * R::P, p, lane);
+      R::cols(acc, Vs + 32 * b * R::P, p, lane);
       if (EXACT) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] = Elem<T>::left(p[r]);
-        R::cols(acc, Vs + 32 * sub * R::P, p, lane);
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) p[r] = Elem<T>::left(p[r]);
+          R::cols(acc, Vs + 32 * b * R::P, p, lane);
+        }
       }
     }
   }
-  l += __shfl_xor(l, 32, 64);
+  l = half_sum(l);
   if (qi >= a.S) return;
   const float inv = real && l > 0.f ? 1.f / l : 0.f;
   const int64_t at = (tok0 + qi) * (int64_t)(a.H * D) + h * D + 4 * hh;
@@ -337,17 +375,15 @@ __global__ __launch_bounds__(64 * NW) void fwd_kernel(const Args a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] = nan ? l : real ? acc[db][4 * c + j] * inv : 0.f;
       Elem<T>::store4((T*)a.o + at + 32 * db + 8 * c, x[0], x[1], x[2], x[3]);
-      if (EXACT)
-        Elem<T>::store4((T*)a.olo + at + 32 * db + 8 * c, Elem<T>::left(x[0]), Elem<T>::left(x[1]),
-                        Elem<T>::left(x[2]), Elem<T>::left(x[3]));
+      if (sizeof(T) == 2 && a.o32) Elem<float>::store4(a.o32 + at + 32 * db + 8 * c, x[0], x[1], x[2], x[3]);
     }
   if (a.lse && hh == 0)
     a.lse[((int64_t)n * a.H + h) * a.S + qi] = nan ? l : real && l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
 }
 
 // ----------------------------------------------------------------------------------------------------------------
-// Backward, dq (and D, dbias): the forward's walk. D_i = dO_i·o_i is formed from the forward's rounded output and
-// what its rounding left over, where dbias (fp32) needs it exact.
+// Backward, dq (and D, dbias): the forward's walk. D_i = dO_i·o_i takes the forward's output as it was before its
+// rounding to bf16: with the rounded one the rows of dS would not sum to zero, half as far off as by dS's own rounding.
 // dbias: dS is summed per distance, in one order whatever the launch: a 32×32 block goes to LDS skewed by its row, so
 // that a column holds one distance, and a lane adds up a column and adds it to the wave's own bin of that distance;
 // blocks whose distances all lie in the last bucket are summed in registers.
@@ -382,16 +418,12 @@ __global__ __launch_bounds__(64 * NW) void dq_kernel(const Args a) {
   R::frags(df, (const T*)a.dout + (tok0 + qi) * a.lddo + h * D, real, hh);
   float Dq = 0.f, L = INFINITY;
   if (real) {
-    const T* op = (const T*)a.o + (tok0 + qi) * (int64_t)(a.H * D) + h * D;
-    const T* lp = a.olo ? (const T*)a.olo + (tok0 + qi) * (int64_t)(a.H * D) + h * D : nullptr;
+    const float* op = a.o32 + (tok0 + qi) * (int64_t)(a.H * D) + h * D;
 #pragma unroll
-    for (int c = 0; c < R::NC; ++c) {
-      Dq = Elem<T>::dot(df[c], R::unit(op, 2 * c + hh), Dq);
-      if (sizeof(T) == 2 && lp) Dq = Elem<T>::dot(df[c], R::unit(lp, 2 * c + hh), Dq);
-    }
+    for (int c = 0; c < R::NC; ++c) Dq = Elem<T>::dot(df[c], op + (2 * c + hh) * R::E, Dq);
     L = a.lse[((int64_t)n * a.H + h) * a.S + qi];
   }
-  Dq += __shfl_xor(Dq, 32, 64);
+  Dq = half_sum(Dq);
   if (qi < a.S && hh == 0) a.dsum[((int64_t)n * a.H + h) * a.S + qi] = Dq;
   if (BIAS) {
     fill_lut(lut, a, n / (a.N / a.C), h, tid, 64 * NW);
@@ -423,13 +455,10 @@ __global__ __launch_bounds__(64 * NW) void dq_kernel(const Args a) {
 #pragma unroll
     for (int sub = 0; sub < BK / 32; ++sub) {
       const int kb = k0 + 32 * sub;
-      if (qw >= a.S || kb >= a.S || kb > qw + 31 || !(qw - kb - 31 < a.W || kb < a.sinks)) continue;
+      if (!block_seen(a, qw, kb)) continue;
       f32x16 s = R::rows(Ks + 32 * sub * R::P, qf, lane);
       const f32x16 dp = R::rows(Vs + 32 * sub * R::P, df, lane);
-      const uint32_t bits =
-          (uint32_t)__ballot(kb + (lane & 31) < a.S && (!mask || mask[kb + (lane & 31)])) >> (4 * hh);
-      const bool all = !__any(bits != (hh ? 0x0fffffffu : 0xffffffffu)) && kb + 31 <= qw &&
-                       (qw + 31 - kb < a.W || kb + 31 < a.sinks);
+      const uint32_t bits = token_bits(a, mask, kb, lane);
       const bool near = BIAS && qw - kb - 31 < a.maxd;
       if (BIAS) {
         if (near) {
@@ -448,11 +477,12 @@ __global__ __launch_bounds__(64 * NW) void dq_kernel(const Args a) {
       float ds[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(s[r]) * (dp[r] - Dq);
-      if (!all) {
+      if (bits != 0xffffffffu || !block_whole(a, qw, kb)) {
+        const uint32_t mine = bits >> (4 * hh);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int key = kb + kappa(r) + 4 * hh;
-          const bool see = key <= qi && (qi - key < a.W || key < a.sinks) && ((bits >> kappa(r)) & 1);
+          const bool see = key <= qi && (qi - key < a.W || key < a.sinks) && ((mine >> kappa(r)) & 1);
           ds[r] = see ? ds[r] : 0.f;
         }
       }
@@ -811,7 +841,7 @@ __global__ __launch_bounds__(64 * NW) void step_kernel(const StepArgs a) {
       float mt = s[0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
-      mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+      mt = half_max(mt);
       const float mn = fmaxf(m, mt), mu = mn == -INFINITY ? 0.f : mn;
       const float al = __builtin_amdgcn_exp2f(m - mu);
       l *= al;
@@ -831,7 +861,7 @@ __global__ __launch_bounds__(64 * NW) void step_kernel(const StepArgs a) {
       __builtin_amdgcn_wave_barrier();
     }
   }
-  l += __shfl_xor(l, 32, 64);
+  l = half_sum(l);
   if (hh == 0) {
     ml[w][0][lane] = m;
     ml[w][1][lane] = l;
@@ -929,8 +959,10 @@ __global__ __launch_bounds__(256) void fill_kernel(const uint4* __restrict__ k, 
 template <typename T, int D, int NW, int BK> int launch_fwd_tile(const Args& a, hipStream_t st) {
   const size_t lds = a.bias ? (a.maxd + 2 * kLutOff) * sizeof(float) : 0;
   const dim3 grid((unsigned)((int64_t)a.N * a.H * ((a.S + 32 * NW - 1) / (32 * NW)))), block(64 * NW);
-  if (sizeof(T) == 2 && a.olo) hipLaunchKernelGGL((fwd_kernel<T, D, NW, BK, sizeof(T) == 2>), grid, block, lds, st, a);
-  else hipLaunchKernelGGL((fwd_kernel<T, D, NW, BK, false>), grid, block, lds, st, a);
+  if (!a.bias) hipLaunchKernelGGL((fwd_kernel<T, D, NW, BK, false, false>), grid, block, 0, st, a);
+  else if (sizeof(T) == 2 && a.exact)
+    hipLaunchKernelGGL((fwd_kernel<T, D, NW, BK, true, sizeof(T) == 2>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((fwd_kernel<T, D, NW, BK, true, false>), grid, block, lds, st, a);
   return (int)hipGetLastError();
 }
 

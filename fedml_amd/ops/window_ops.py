@@ -30,10 +30,10 @@ _I32 = 2 ** 31 - 1
 
 
 class _Args(_c.Structure):
-    _fields_ = [(n, _c.c_void_p) for n in ("q", "k", "v", "dout", "o", "olo", "dq", "dk", "dv", "lse", "dsum", "part",
+    _fields_ = [(n, _c.c_void_p) for n in ("q", "k", "v", "dout", "o", "dq", "dk", "dv", "o32", "lse", "dsum", "part",
                                            "bpart", "dbias", "mask", "bias")] + \
                [(n, _c.c_int64) for n in ("ldq", "ldk", "ldv", "lddo")] + \
-               [(n, _c.c_int) for n in ("N", "S", "H", "KV", "C", "W", "sinks", "NB", "maxd", "nchunk", "qchunk")] + \
+               [(n, _c.c_int) for n in ("N", "S", "H", "KV", "C", "W", "sinks", "NB", "maxd", "nchunk", "qchunk", "exact")] + \
                [("scale", _c.c_float), ("start", _c.c_int * MAX_BUCKETS)]
 
 
@@ -123,7 +123,10 @@ def _bias(bias, sequences, H, max_distance, device):
 
 
 def _scale(scale, D):
-    return 1.0 / math.sqrt(D) if scale is None else float(scale)
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"scale > 0 expected, got {scale}")
+    return scale
 
 
 def _aligned(t):
@@ -190,16 +193,18 @@ def _args(q, k, v, mask, bias, starts, cfg):
 
 
 def _forward(q, k, v, mask, bias, starts, cfg, keep, exact):
-    """(o, what its rounding left over, log-sum-exp); keep: for a backward pass, exact: with a gradient of the bias."""
+    """(o, o before its rounding, log-sum-exp); keep: for a backward pass, exact: with a gradient of the bias."""
     S, H, D = cfg[0], cfg[1], cfg[5]
     o = torch.empty(q.shape[0], H * D, dtype=q.dtype, device=q.device)
-    olo = torch.empty_like(o) if exact and q.dtype == torch.bfloat16 else None
-    lse = torch.empty(q.shape[0] // S, H, S, dtype=torch.float32, device=q.device) if keep else None
+    o32 = lse = None
+    if keep:
+        o32 = o if q.dtype == torch.float32 else torch.empty(o.shape, dtype=torch.float32, device=q.device)
+        lse = torch.empty(q.shape[0] // S, H, S, dtype=torch.float32, device=q.device)
     if q.shape[0]:
         a = _args(q, k, v, mask, bias, starts, cfg)
-        a.o, a.olo, a.lse = _v(_p(o)), _v(_p(olo)), _v(_p(lse))
+        a.o, a.o32, a.lse, a.exact = _v(_p(o)), _v(_p(o32)), _v(_p(lse)), int(exact)
         _launch("fa_window_fwd", a, q.dtype, D, q)
-    return o, olo, lse
+    return o, o32, lse
 
 
 class _WindowAttention(torch.autograd.Function):
@@ -207,15 +212,15 @@ class _WindowAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, bias, mask, starts, cfg):
         q, k, v = _aligned(q), _aligned(k), _aligned(v)
         tab = None if bias is None else bias.contiguous()
-        o, olo, lse = _forward(q, k, v, mask, tab, starts, cfg, True, bias is not None and ctx.needs_input_grad[3])
-        ctx.save_for_backward(q, k, v, tab, mask, o, olo, lse)
+        o, o32, lse = _forward(q, k, v, mask, tab, starts, cfg, True, bias is not None and ctx.needs_input_grad[3])
+        ctx.save_for_backward(q, k, v, tab, mask, o32, lse)
         ctx.starts, ctx.cfg = starts, cfg
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, bias, mask, o, olo, lse = ctx.saved_tensors
+        q, k, v, bias, mask, o32, lse = ctx.saved_tensors
         S, H, KV, W, sinks, D, _, _ = ctx.cfg
         N, dev = q.shape[0] // S, q.device
         do = _aligned(do.to(q.dtype))
@@ -234,7 +239,7 @@ class _WindowAttention(torch.autograd.Function):
                 part = torch.empty(N, KV, a.nchunk + 1, 2, sinks, D, dtype=torch.float32, device=dev)
             if dbias is not None:
                 bpart = torch.empty(N, H, -(-S // tile), bias.shape[-1], dtype=torch.float32, device=dev)
-            a.dout, a.lddo, a.lse, a.o, a.olo = _v(_pr(do)), do.stride(0), _v(_pr(lse)), _v(_pr(o)), _v(_pr(olo))
+            a.dout, a.lddo, a.lse, a.o32 = _v(_pr(do)), do.stride(0), _v(_pr(lse)), _v(_pr(o32))
             a.dq, a.dk, a.dv, a.dsum = _v(_p(dq)), _v(_p(dk)), _v(_p(dv)), _v(_p(dsum))
             a.part, a.bpart, a.dbias = _v(_p(part)), _v(_p(bpart)), _v(_p(dbias))
             _launch("fa_window_bwd", a, q.dtype, D, q)

@@ -160,6 +160,7 @@ def _t(*shape, dtype=torch.float32):
     (TypeError, "bf16 or fp32", dict(q=_t(8, 128, dtype=torch.float16))),
     (ValueError, "whole sequences", dict(S=3)), (ValueError, "whole sequences", dict(S=0)),
     (ValueError, "window", dict(window=0)), (ValueError, "sinks", dict(sinks=-1)), (ValueError, "sinks", dict(sinks=65)),
+    (ValueError, "scale", dict(scale=0.0)), (ValueError, "scale", dict(scale=float("nan"))),
     (ValueError, "mask", dict(mask=_t(2, 4))), (ValueError, "mask", dict(mask=torch.ones(2, 3, dtype=torch.bool))),
     (ValueError, "bias", dict(bias=_t(3, 8))), (TypeError, "bias", dict(bias=_t(2, 8, dtype=torch.bfloat16))),
     (ValueError, "clients", dict(bias=_t(3, 2, 8))), (ValueError, "buckets", dict(bias=_t(2, 1))),

@@ -389,7 +389,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void fwd_kernel(const Arg
 // blocks whose distances all lie in the last bucket are summed in registers.
 // ----------------------------------------------------------------------------------------------------------------
 template <typename T, int D, int NW, int BK, bool BIAS>
-__global__ __launch_bounds__(64 * NW) void dq_kernel(const Args a) {
+__global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void dq_kernel(const Args a) {
   using R = Row<T, D>;
   __shared__ __attribute__((aligned(16))) T Ks[BK * R::P];
   __shared__ __attribute__((aligned(16))) T Vs[BK * R::P];
@@ -544,7 +544,7 @@ __global__ __launch_bounds__(64 * NW) void dq_kernel(const Args a) {
 // order (the sinks' own rows of the window pass among them).
 // ----------------------------------------------------------------------------------------------------------------
 template <typename T, int D, int NW, int BQ>
-__global__ __launch_bounds__(64 * NW) void dkv_kernel(const Args a) {
+__global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kernel(const Args a) {
   using R = Row<T, D>;
   __shared__ __attribute__((aligned(16))) T Qs[BQ * R::P];
   __shared__ __attribute__((aligned(16))) T Os[BQ * R::P];
@@ -985,7 +985,7 @@ template <typename T, int D, int NW, int BK> int launch_dq(const Args& a, hipStr
 template <typename T, int D> int launch_bwd(const Args& a, hipStream_t st) {
   const size_t lds = a.bias ? (a.maxd + 2 * kLutOff) * sizeof(float) : 0;
   int rc;
-  if (a.S > 64) rc = launch_dq<T, D, 4, 32>(a, st);
+  if (a.S > 64) rc = launch_dq<T, D, 4, sizeof(T) == 2 ? 64 : 32>(a, st);
   else rc = launch_dq<T, D, 1, 32>(a, st);
   if (rc) return rc;
   const int64_t nsink = (int64_t)a.nchunk * a.N * a.KV;
@@ -993,7 +993,7 @@ template <typename T, int D> int launch_bwd(const Args& a, hipStream_t st) {
   constexpr int kFew = D * sizeof(T) > 256 ? 4 : 2;
   if (a.S > 64) {
     const int64_t n = nsink + (int64_t)a.N * a.KV * ((a.S + 127) / 128);
-    hipLaunchKernelGGL((dkv_kernel<T, D, 4, 32>), dim3((unsigned)n), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((dkv_kernel<T, D, 4, sizeof(T) == 2 ? 64 : 32>), dim3((unsigned)n), dim3(256), lds, st, a);
   } else {
     const int64_t n = nsink + (int64_t)a.N * a.KV;
     hipLaunchKernelGGL((dkv_kernel<T, D, kFew, 32>), dim3((unsigned)n), dim3(64 * kFew), lds, st, a);

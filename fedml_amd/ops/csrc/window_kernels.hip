@@ -29,7 +29,8 @@ typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 8.f;      // see fwd_kernel
 constexpr int kMaxBuckets = 128;
-constexpr int kLutOff = 62;      // a processed 32×32 block holds distances >= −62 (the negative ones are masked)
+constexpr int kLutOff = 94;      // a processed block of 32 queries and <= 64 keys holds distances >= −94 (the negative
+                                 // ones are masked), and below max_distance + 94 if it holds one below max_distance
 constexpr int kBinPad = 64;      // distances of a block that starts below max_distance end below max_distance + 62
 
 struct Args {
@@ -57,7 +58,6 @@ __device__ __forceinline__ int xcd_swizzle(int id, int n) {
 
 template <typename T> struct Elem;
 template <> struct Elem<uint16_t> {
-  static constexpr int kPad = 8;
   static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                    0, 0);
@@ -84,7 +84,6 @@ template <> struct Elem<uint16_t> {
   static __device__ __forceinline__ float left(float a) { return a - bf16_to_f32(f32_to_bf16(a)); }
 };
 template <> struct Elem<float> {
-  static constexpr int kPad = 4;
   static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
     const float4 x = __builtin_bit_cast(float4, a), y = __builtin_bit_cast(float4, b);
     c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, y.x, c, 0, 0, 0);
@@ -109,6 +108,14 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
+// A matrix instruction's result may be read 19 instruction slots after its issue (16 passes; 11 for 8). The compiler
+// inserts what is missing, but has been seen to count the longer of two branches between the product and the first use
+// (the last accumulator of 16 was read 11 slots early): wait here, in the product's own block.
+__device__ __forceinline__ void settle(f32x16& a) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a)); }
+__device__ __forceinline__ void settle(f32x16& a, f32x16& b) {
+  asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a), "+v"(b));
+}
+
 // over the two halves of the wave (which hold the same column)
 __device__ __forceinline__ float half_max(float v) {
   const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -119,17 +126,22 @@ __device__ __forceinline__ float half_sum(float v) {
   return __uint_as_float(x[0]) + __uint_as_float(x[1]);
 }
 
-// What a 32×32 block of scores (queries from q, keys from k) is to a wave: seen at all, seen whole
-__device__ __forceinline__ bool block_seen(const Args& a, int q, int k) {
-  return q < a.S && k < a.S && k <= q + 31 && (q - k - 31 < a.W || k < a.sinks);
+// What a block of scores (32 queries from q, nk keys from k) is to a wave: seen at all, seen whole
+__device__ __forceinline__ bool block_seen(const Args& a, int q, int k, int nk) {
+  return q < a.S && k < a.S && k <= q + 31 && (q - k - nk + 1 < a.W || k < a.sinks);
 }
-__device__ __forceinline__ bool block_whole(const Args& a, int q, int k) {
-  return k + 31 <= q && (q + 31 - k < a.W || k + 31 < a.sinks);
+__device__ __forceinline__ bool block_whole(const Args& a, int q, int k, int nk) {
+  return k + nk - 1 <= q && (q + 31 - k < a.W || k + nk - 1 < a.sinks);
 }
-// bit j: key k0 + j is a token, for the 32 keys of a block
-__device__ __forceinline__ uint32_t token_bits(const Args& a, const uint8_t* mask, int k0, int lane) {
-  const int key = k0 + (lane & 31);
-  return (uint32_t)__ballot(key < a.S && (!mask || mask[key]));
+
+// lane j of ROWS: is row r0 + j < end a token (their ballot: a tile's bits)
+template <int ROWS> __device__ __forceinline__ int token(const uint8_t* mask, int r0, int end, int lane) {
+  const int r = r0 + lane % ROWS;
+  const int m = mask ? mask[r < end ? r : end - 1] : 1;
+  return r < end ? m : 0;
+}
+template <int ROWS> __device__ __forceinline__ uint64_t token_bits(int tok) {
+  return (uint64_t)__ballot(tok != 0) & (~0ull >> (64 - ROWS));
 }
 
 // A head's rows and how they lie in registers and LDS
@@ -137,8 +149,40 @@ template <typename T, int D> struct Row {
   static constexpr int U = D * (int)sizeof(T) / 16;   // 16-byte units of a row
   static constexpr int NC = U / 2;                    // chunks: a unit for either half of the wave
   static constexpr int E = 16 / (int)sizeof(T);       // elements of a unit
-  static constexpr int P = D + Elem<T>::kPad;         // LDS pitch: 16 rows' units lie on different banks
   static constexpr int DB = D / 32;                   // 32-column blocks
+
+  // LDS tiles. fp32: rows padded by 16 bytes. bf16: row r has its unit u at unit u ^ swz(r), and swz runs over the units
+  // with 16 rows, so the 16 lanes that a ds_read_b128 serves at once meet 64 different banks, and the 4 rows of a
+  // transposing read lie 4 units apart (padded rows cost its reads at D 128 2.5 times their cycles).
+  static constexpr int P = sizeof(T) == 4 ? D + 4 : D;
+  static __device__ __forceinline__ int swz(int r) {
+    if constexpr (sizeof(T) == 4) return 0;
+    else if constexpr (D == 64) return ((r & 2) << 1) | ((r >> 2) & 3);
+    else return ((r & 3) << 2) | ((r >> 2) & 3);
+  }
+  static __device__ __forceinline__ int at(int r, int u) { return r * P + (u ^ swz(r)) * E; }
+  // a lane's places in 32 rows of any tile, as row operand (by chunk) and as column operand (by column block and row
+  // half); kept in registers as they are, so that tiles and blocks are constant offsets from them
+  struct Lane {
+    int row[NC], col[sizeof(T) == 4 ? 1 : 2 * (D / 32)];
+    __device__ __forceinline__ explicit Lane(int lane) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) row[c] = at(lane & 31, 2 * c + (lane >> 5));
+      if constexpr (sizeof(T) == 4) {
+        col[0] = 4 * (lane >> 5) * P + (lane & 31);
+      } else {
+        // 16 lanes read 4 rows × 16 columns and get a column of 4 rows each
+        const int g = lane >> 4, i = lane & 15;
+#pragma unroll
+        for (int k = 0; k < 2 * DB; ++k) {
+          col[k] = at(4 * (g >> 1) + (i >> 2) + 8 * (k & 1), 4 * (k >> 1) + 2 * (g & 1) + ((i & 3) >> 1)) + 4 * (i & 1);
+          asm volatile("" : "+v"(col[k]));
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) asm volatile("" : "+v"(row[c]));
+      }
+    }
+  };
 
   static __device__ __forceinline__ uint4 unit(const T* row, int u) {
     return *reinterpret_cast<const uint4*>(row + u * E);
@@ -149,31 +193,27 @@ template <typename T, int D> struct Row {
     for (int c = 0; c < NC; ++c) f[c] = real ? unit(row, 2 * c + hh) : make_uint4(0, 0, 0, 0);
   }
   // 32 rows of an LDS tile × this lane's column: Σ over the head dim
-  static __device__ __forceinline__ f32x16 rows(const T* tile, const uint4* f, int lane) {
+  static __device__ __forceinline__ f32x16 rows(const T* tile, const uint4* f, const Lane& ln) {
     f32x16 acc = zero16();
-    const T* row = tile + (lane & 31) * P;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) acc = Elem<T>::mma(unit(row, 2 * c + (lane >> 5)), f[c], acc);
+    for (int c = 0; c < NC; ++c) acc = Elem<T>::mma(*reinterpret_cast<const uint4*>(tile + ln.row[c]), f[c], acc);
     return acc;
   }
   // acc[db][column][row] += Σ over 32 rows of the LDS tile of tile[row][32 db + ·] · p[row]
-  static __device__ __forceinline__ void cols(f32x16* acc, const T* tile, const float* p, int lane) {
+  static __device__ __forceinline__ void cols(f32x16* acc, const T* tile, const float* p, const Lane& ln) {
     if constexpr (sizeof(T) == 2) {
       bf16x8 b[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int j = 0; j < 8; ++j) b[t][j] = (__bf16)p[8 * t + j];
-      const int g = lane >> 4, i = lane & 15;
-      // 16 lanes read 4 rows × 16 columns and get a column of 4 rows each
-      const uint16_t* at = reinterpret_cast<const uint16_t*>(tile) + (4 * (g >> 1) + (i >> 2)) * P + 16 * (g & 1) +
-                           4 * (i & 3);
+      const uint16_t* base = reinterpret_cast<const uint16_t*>(tile);
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const v4i16 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(at + 16 * t * P + 32 * db));
-          const v4i16 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(at + (16 * t + 8) * P + 32 * db));
+        for (int t = 0; t < 2; ++t) {      // swz(row + 16) = swz(row)
+          const v4i16 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(base + 16 * t * P + ln.col[2 * db]));
+          const v4i16 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(base + 16 * t * P + ln.col[2 * db + 1]));
           union {
             v4i16 h[2];
             bf16x8 v;
@@ -183,41 +223,46 @@ template <typename T, int D> struct Row {
           acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b[t], acc[db], 0, 0, 0);
         }
     } else {
-      const float* at = reinterpret_cast<const float*>(tile) + 4 * (lane >> 5) * P + (lane & 31);
+      const float* base = reinterpret_cast<const float*>(tile) + ln.col[0];
 #pragma unroll
       for (int r = 0; r < 16; ++r)
 #pragma unroll
         for (int db = 0; db < DB; ++db)
-          acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[kappa(r) * P + 32 * db], p[r], acc[db], 0, 0, 0);
+          acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(base[kappa(r) * P + 32 * db], p[r], acc[db], 0, 0, 0);
     }
   }
 };
 
-// ROWS rows of a [·][D] source between registers and an LDS tile, NT threads; rows that are no tokens become zero, so
-// that what they hold (NaN included) reaches no product
+// ROWS rows of a [·][D] source between registers and an LDS tile, NT threads. Loads are unconditional, of rows up to
+// `last`; a row without its bit in `bits` (no token, or behind the last) is zero in the tile, so that what it holds (NaN
+// included) reaches no product.
 template <typename T, int D, int ROWS, int NT> struct Stage {
   using R = Row<T, D>;
   static constexpr int NI = ROWS * R::U / NT;
-  static_assert(NI >= 1 && ROWS * R::U % NT == 0, "staging");
+  static_assert(NI >= 1 && ROWS * R::U % NT == 0 && ROWS <= 64, "staging");
   uint4 reg[NI];
-  __device__ __forceinline__ void load(const T* src, int64_t ld, int row0, int end, const uint8_t* mask, int tid) {
+  __device__ __forceinline__ void load(const T* src, int64_t ld, int row0, int last, int tid) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int u = tid + i * NT, row = row0 + u / R::U;
-      reg[i] = make_uint4(0, 0, 0, 0);
-      if (row < end && (!mask || mask[row])) reg[i] = R::unit(src + row * ld, u % R::U);
+      reg[i] = R::unit(src + (row < last ? row : last) * ld, u % R::U);
     }
   }
-  __device__ __forceinline__ void store(T* tile, int tid) const {
+  __device__ __forceinline__ void store(T* tile, uint64_t bits, int tid) {
+    if (bits != ~0ull >> (64 - ROWS)) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        if (!((bits >> ((tid + i * NT) / R::U)) & 1)) reg[i] = make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int u = tid + i * NT;
-      *reinterpret_cast<uint4*>(tile + (u / R::U) * R::P + (u % R::U) * R::E) = reg[i];
+      *reinterpret_cast<uint4*>(tile + R::at(u / R::U, u % R::U)) = reg[i];
     }
   }
 };
 
-// lut[d + kLutOff] = bias of distance d in units of log 2, for −62 <= d < max_distance + 62
+// lut[d + kLutOff] = bias of distance d in units of log 2, for −94 <= d < max_distance + 94
 __device__ __forceinline__ int lut_size(int maxd) { return maxd + 2 * kLutOff; }
 __device__ __forceinline__ void fill_lut(float* lut, const Args& a, int client, int h, int tid, int nt) {
   const float* tab = a.bias + ((int64_t)client * a.H + h) * a.NB;
@@ -255,6 +300,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void fwd_kernel(const Arg
   __shared__ __attribute__((aligned(16))) T Vs[BK * R::P];
   extern __shared__ float lut[];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
+  const typename R::Lane ln(lane);
   const int G = a.H / a.KV, nqt = (a.S + 32 * NW - 1) / (32 * NW);
   int id = xcd_swizzle(blockIdx.x, gridDim.x);
   const int g = id % G;
@@ -279,56 +325,63 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void fwd_kernel(const Arg
 #pragma unroll
   for (int db = 0; db < R::DB; ++db) acc[db] = zero16();
   Stage<T, D, BK, 64 * NW> sk, sv;
+  int tok = 0;
   if (count) {
-    sk.load(kp, a.ldk, tiles.at(0) * BK, a.S, mask, tid);
-    sv.load(vp, a.ldv, tiles.at(0) * BK, a.S, mask, tid);
+    tok = token<BK>(mask, tiles.at(0) * BK, a.S, lane);
+    sk.load(kp, a.ldk, tiles.at(0) * BK, a.S - 1, tid);
+    sv.load(vp, a.ldv, tiles.at(0) * BK, a.S - 1, tid);
   }
   for (int it = 0; it < count; ++it) {
     const int k0 = tiles.at(it) * BK;
     __syncthreads();
-    sk.store(Ks, tid);
-    sv.store(Vs, tid);
+    const uint64_t bits = token_bits<BK>(tok);
+    sk.store(Ks, bits, tid);
+    sv.store(Vs, bits, tid);
     __syncthreads();
     if (it + 1 < count) {
-      sk.load(kp, a.ldk, tiles.at(it + 1) * BK, a.S, mask, tid);
-      sv.load(vp, a.ldv, tiles.at(it + 1) * BK, a.S, mask, tid);
+      tok = token<BK>(mask, tiles.at(it + 1) * BK, a.S, lane);
+      sk.load(kp, a.ldk, tiles.at(it + 1) * BK, a.S - 1, tid);
+      sv.load(vp, a.ldv, tiles.at(it + 1) * BK, a.S - 1, tid);
     }
     constexpr int NB = BK / 32;
+    if (!block_seen(a, qw, k0, BK)) continue;
     f32x16 s[NB];
-    bool seen[NB], any = false;
-    float mt = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int kb = k0 + 32 * b;
-      seen[b] = block_seen(a, qw, kb);
-      if (!seen[b]) continue;
-      any = true;
-      s[b] = R::rows(Ks + 32 * b * R::P, qf, lane);
-      const uint32_t bits = token_bits(a, mask, kb, lane);
-      if (BIAS) {
-        if (qw - kb - 31 < a.maxd) {
-          const float* at = lut + kLutOff + qi - kb - 4 * hh;
+    for (int b = 0; b < NB; ++b) s[b] = R::rows(Ks + 32 * b * R::P, qf, ln);
+    if constexpr (NB == 2) settle(s[0], s[1]);
+    else settle(s[0]);
+    if (BIAS) {
+      if (qw - k0 - (BK - 1) < a.maxd) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const float* at = lut + kLutOff + qi - k0 - 32 * b - 4 * hh;
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], c2, at[-kappa(r)]);
-        } else {
-          const float far = lut[lut_size(a.maxd) - 1];
+        }
+      } else {
+        const float far = lut[lut_size(a.maxd) - 1];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], c2, far);
-        }
       }
-      if (bits != 0xffffffffu || !block_whole(a, qw, kb)) {
-        const uint32_t mine = bits >> (4 * hh);
+    }
+    if (bits != ~0ull >> (64 - BK) || !block_whole(a, qw, k0, BK)) {
+      const uint64_t mine = bits >> (4 * hh);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int key = kb + kappa(r) + 4 * hh;
-          const bool see = key <= qi && (qi - key < a.W || key < a.sinks) && ((mine >> kappa(r)) & 1);
+          const int key = k0 + 32 * b + kappa(r) + 4 * hh;
+          const bool see = key <= qi && (qi - key < a.W || key < a.sinks) && ((mine >> (32 * b + kappa(r))) & 1);
           s[b][r] = see ? s[b][r] : -INFINITY;
         }
-      }
+    }
+    float mt = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[b][r]);
-    }
-    if (!any) continue;
     mt = half_max(mt);
     if (!BIAS) mt *= c2;
     if (__any(mt > m + kGrow)) {
@@ -344,24 +397,25 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void fwd_kernel(const Arg
     const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      if (!seen[b]) continue;
       float p[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         p[r] = __builtin_amdgcn_exp2f(BIAS ? s[b][r] - mu : fmaf(s[b][r], c2, -mu));
         l += p[r];
       }
-      R::cols(acc, Vs + 32 * b * R::P, p, lane);
+      R::cols(acc, Vs + 32 * b * R::P, p, ln);
       if (EXACT) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) p[r] = Elem<T>::left(p[r]);
-          R::cols(acc, Vs + 32 * b * R::P, p, lane);
+          R::cols(acc, Vs + 32 * b * R::P, p, ln);
         }
       }
     }
   }
+#pragma unroll
+  for (int db = 0; db < R::DB; ++db) settle(acc[db]);
   l = half_sum(l);
   if (qi >= a.S) return;
   const float inv = real && l > 0.f ? 1.f / l : 0.f;
@@ -389,7 +443,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void fwd_kernel(const Arg
 // blocks whose distances all lie in the last bucket are summed in registers.
 // ----------------------------------------------------------------------------------------------------------------
 template <typename T, int D, int NW, int BK, bool BIAS>
-__global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void dq_kernel(const Args a) {
+__global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) void dq_kernel(const Args a) {
   using R = Row<T, D>;
   __shared__ __attribute__((aligned(16))) T Ks[BK * R::P];
   __shared__ __attribute__((aligned(16))) T Vs[BK * R::P];
@@ -397,6 +451,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void dq_kernel(const Args
   __shared__ float fars[NW];
   extern __shared__ float lut[];                 // BIAS: lut, then NW × (maxd + kBinPad) bins
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
+  const typename R::Lane ln(lane);
   const int G = a.H / a.KV, nqt = (a.S + 32 * NW - 1) / (32 * NW);
   int id = xcd_swizzle(blockIdx.x, gridDim.x);
   const int g = id % G;
@@ -438,27 +493,33 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void dq_kernel(const Args
 #pragma unroll
   for (int db = 0; db < R::DB; ++db) acc[db] = zero16();
   Stage<T, D, BK, 64 * NW> sk, sv;
+  int tok = 0;
   if (count) {
-    sk.load(kp, a.ldk, tiles.at(0) * BK, a.S, mask, tid);
-    sv.load(vp, a.ldv, tiles.at(0) * BK, a.S, mask, tid);
+    tok = token<BK>(mask, tiles.at(0) * BK, a.S, lane);
+    sk.load(kp, a.ldk, tiles.at(0) * BK, a.S - 1, tid);
+    sv.load(vp, a.ldv, tiles.at(0) * BK, a.S - 1, tid);
   }
   for (int it = 0; it < count; ++it) {
     const int k0 = tiles.at(it) * BK;
     __syncthreads();
-    sk.store(Ks, tid);
-    sv.store(Vs, tid);
+    const uint64_t bits = token_bits<BK>(tok);
+    sk.store(Ks, bits, tid);
+    sv.store(Vs, bits, tid);
     __syncthreads();
     if (it + 1 < count) {
-      sk.load(kp, a.ldk, tiles.at(it + 1) * BK, a.S, mask, tid);
-      sv.load(vp, a.ldv, tiles.at(it + 1) * BK, a.S, mask, tid);
+      tok = token<BK>(mask, tiles.at(it + 1) * BK, a.S, lane);
+      sk.load(kp, a.ldk, tiles.at(it + 1) * BK, a.S - 1, tid);
+      sv.load(vp, a.ldv, tiles.at(it + 1) * BK, a.S - 1, tid);
     }
+    if (!block_seen(a, qw, k0, BK)) continue;
+    const bool whole = bits == ~0ull >> (64 - BK) && block_whole(a, qw, k0, BK);
 #pragma unroll
     for (int sub = 0; sub < BK / 32; ++sub) {
       const int kb = k0 + 32 * sub;
-      if (!block_seen(a, qw, kb)) continue;
-      f32x16 s = R::rows(Ks + 32 * sub * R::P, qf, lane);
-      const f32x16 dp = R::rows(Vs + 32 * sub * R::P, df, lane);
-      const uint32_t bits = token_bits(a, mask, kb, lane);
+      if (!block_seen(a, qw, kb, 32)) continue;
+      f32x16 s = R::rows(Ks + 32 * sub * R::P, qf, ln);
+      f32x16 dp = R::rows(Vs + 32 * sub * R::P, df, ln);
+      settle(s, dp);
       const bool near = BIAS && qw - kb - 31 < a.maxd;
       if (BIAS) {
         if (near) {
@@ -477,8 +538,8 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void dq_kernel(const Args
       float ds[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(s[r]) * (dp[r] - Dq);
-      if (bits != 0xffffffffu || !block_whole(a, qw, kb)) {
-        const uint32_t mine = bits >> (4 * hh);
+      if (!whole) {
+        const uint32_t mine = (uint32_t)(bits >> (32 * sub)) >> (4 * hh);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int key = kb + kappa(r) + 4 * hh;
@@ -486,7 +547,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void dq_kernel(const Args
           ds[r] = see ? ds[r] : 0.f;
         }
       }
-      R::cols(acc, Ks + 32 * sub * R::P, ds, lane);
+      R::cols(acc, Ks + 32 * sub * R::P, ds, ln);
       if (BIAS) {
         if (near) {
           float* at = sk_w + (lane & 31) * 65 + 31 - 4 * hh;       // row i, column i − key + 31
@@ -508,6 +569,8 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void dq_kernel(const Args
       }
     }
   }
+#pragma unroll
+  for (int db = 0; db < R::DB; ++db) settle(acc[db]);
   if (qi < a.S) {
     T* out = (T*)a.dq + (tok0 + qi) * (int64_t)(a.H * D) + h * D + 4 * hh;
 #pragma unroll
@@ -551,6 +614,7 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
   __shared__ __attribute__((aligned(16))) float Ls[BQ], Ds[BQ];
   extern __shared__ float lut[];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
+  const typename R::Lane ln(lane);
   const int G = a.H / a.KV, nkt = (a.S + 32 * NW - 1) / (32 * NW);
   const int nsink = a.nchunk * a.N * a.KV;
   const bool sink = (int)blockIdx.x < nsink;
@@ -582,11 +646,13 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
 #pragma unroll
   for (int db = 0; db < R::DB; ++db) ak[db] = av[db] = zero16();
   Stage<T, D, BQ, 64 * NW> sq, so;
+  int tok = 0;
   float sl = 0.f, sd = 0.f;                        // threads below BQ: the row's statistics
   auto load = [&](int it) {
     const int h = kv * G + it / nt, q0 = qs + (it % nt) * BQ;
-    sq.load((const T*)a.q + tok0 * a.ldq + h * D, a.ldq, q0, qe, mask, tid);
-    so.load((const T*)a.dout + tok0 * a.lddo + h * D, a.lddo, q0, qe, mask, tid);
+    tok = token<BQ>(mask, q0, qe, lane);
+    sq.load((const T*)a.q + tok0 * a.ldq + h * D, a.ldq, q0, qe - 1, tid);
+    so.load((const T*)a.dout + tok0 * a.lddo + h * D, a.lddo, q0, qe - 1, tid);
     if (tid < BQ) {
       const int64_t at = ((int64_t)n * a.H + h) * a.S + q0 + tid;
       sl = q0 + tid < qe ? a.lse[at] : INFINITY;   // a masked query's is +inf, its D zero
@@ -597,8 +663,9 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
   for (int it = 0; it < count; ++it) {
     const int q0 = qs + (it % nt) * BQ;
     __syncthreads();
-    sq.store(Qs, tid);
-    so.store(Os, tid);
+    const uint64_t bits = token_bits<BQ>(tok);
+    sq.store(Qs, bits, tid);
+    so.store(Os, bits, tid);
     if (tid < BQ) {
       Ls[tid] = sl;
       Ds[tid] = sd;
@@ -606,14 +673,15 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
     if (a.bias && it % nt == 0) fill_lut(lut, a, n / (a.N / a.C), kv * G + it / nt, tid, 64 * NW);
     __syncthreads();
     if (it + 1 < count) load(it + 1);
+    const bool whole = allreal && (sink ? q0 - kw - 31 >= a.W : q0 >= kw + 31 && q0 + BQ - 1 - kw < a.W);
 #pragma unroll
     for (int sub = 0; sub < BQ / 32; ++sub) {
       const int qb = q0 + 32 * sub;
       if (kw >= a.S || qb >= qe || qb + 31 < kw) continue;
       if (sink ? (kw >= a.sinks || qb + 31 - kw < a.W) : qb - kw - 31 >= a.W) continue;
-      const bool all = allreal && (sink ? qb - kw - 31 >= a.W : qb >= kw + 31 && qb + 31 - kw < a.W);
-      f32x16 s = R::rows(Qs + 32 * sub * R::P, kf, lane);
-      const f32x16 dp = R::rows(Os + 32 * sub * R::P, vf, lane);
+      f32x16 s = R::rows(Qs + 32 * sub * R::P, kf, ln);
+      f32x16 dp = R::rows(Os + 32 * sub * R::P, vf, ln);
+      settle(s, dp);
       if (a.bias) {
         if (qb - kw - 31 < a.maxd) {
           const float* at = lut + kLutOff + qb - kj + 4 * hh;
@@ -624,9 +692,6 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, far);
         }
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= c2;
       }
       float p[16], ds[16];
 #pragma unroll
@@ -636,11 +701,12 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
         const float Lr[4] = {L4.x, L4.y, L4.z, L4.w}, Dr[4] = {D4.x, D4.y, D4.z, D4.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          p[4 * c + j] = __builtin_amdgcn_exp2f(s[4 * c + j] - Lr[j]);
-          ds[4 * c + j] = p[4 * c + j] * (dp[4 * c + j] - Dr[j]);
+          const int r = 4 * c + j;
+          p[r] = __builtin_amdgcn_exp2f(a.bias ? s[r] - Lr[j] : fmaf(s[r], c2, -Lr[j]));
+          ds[r] = p[r] * (dp[r] - Dr[j]);
         }
       }
-      if (!all) {
+      if (!whole) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int d = qb + kappa(r) + 4 * hh - kj;
@@ -649,10 +715,12 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
           ds[r] = see ? ds[r] : 0.f;
         }
       }
-      R::cols(av, Os + 32 * sub * R::P, p, lane);
-      R::cols(ak, Qs + 32 * sub * R::P, ds, lane);
+      R::cols(av, Os + 32 * sub * R::P, p, ln);
+      R::cols(ak, Qs + 32 * sub * R::P, ds, ln);
     }
   }
+#pragma unroll
+  for (int db = 0; db < R::DB; ++db) settle(ak[db], av[db]);
   if (kj >= a.S || (sink && kj >= a.sinks)) return;
   if (a.nchunk && kj < a.sinks) {
     float* pk = a.part + ((((int64_t)n * a.KV + kv) * (a.nchunk + 1) + (sink ? chunk + 1 : 0)) * 2 * a.sinks + kj) * D +
@@ -758,6 +826,7 @@ __global__ __launch_bounds__(64 * NW) void step_kernel(const StepArgs a) {
   __shared__ float ml[NW][2][32];
   extern __shared__ float tab[];                  // bias: [heads of the group][NB], then bytes: bucket of a distance
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
+  const typename R::Lane ln(lane);
   const int G = a.H / a.KV, groups = (G + 31) / 32;
   int id = blockIdx.x;
   const int split = id % a.splits;
@@ -823,13 +892,14 @@ __global__ __launch_bounds__(64 * NW) void step_kernel(const StepArgs a) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int u = lane + 64 * i;
-        *reinterpret_cast<uint4*>(Ks + (u / R::U) * R::P + (u % R::U) * R::E) = rk[i];
-        *reinterpret_cast<uint4*>(Vs + (u / R::U) * R::P + (u % R::U) * R::E) = rv[i];
+        *reinterpret_cast<uint4*>(Ks + R::at(u / R::U, u % R::U)) = rk[i];
+        *reinterpret_cast<uint4*>(Vs + R::at(u / R::U, u % R::U)) = rv[i];
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
       if (base + 32 * NW < s1) load(base + 32 * NW);
-      f32x16 s = R::rows(Ks, qf, lane);
+      f32x16 s = R::rows(Ks, qf, ln);
+      settle(s);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int slot = base + kappa(r) + 4 * hh;
@@ -856,11 +926,13 @@ __global__ __launch_bounds__(64 * NW) void step_kernel(const StepArgs a) {
         p[r] = __builtin_amdgcn_exp2f(s[r] - mu);
         l += p[r];
       }
-      R::cols(acc, Vs, p, lane);
+      R::cols(acc, Vs, p, ln);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
   }
+#pragma unroll
+  for (int db = 0; db < R::DB; ++db) settle(acc[db]);
   l = half_sum(l);
   if (hh == 0) {
     ml[w][0][lane] = m;

@@ -1,0 +1,32 @@
+"""Launches of kernels that take their arguments as one structure: small calls are bound by the host, so pointers are
+plain integers and the constant part of a structure is made once per shape and copied."""
+import ctypes as _c
+
+import torch
+
+from . import fl_ops
+
+
+def ptr(t):
+    """Address of an operand the kernel writes (None: null)."""
+    if t is None or fl_ops._SC is None:
+        return None if t is None else t.data_ptr()
+    return fl_ops._p(t).value
+
+
+def ptr_read(t):
+    """Address of an operand the kernel only reads (None: null)."""
+    if t is None or fl_ops._SC is None:
+        return None if t is None else t.data_ptr()
+    return fl_ops._pr(t).value
+
+
+def launch(name, args, ints, device):
+    """Calls ``name(&args, *ints, stream)`` on the device's current stream."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fl_ops._fn(name)(_c.byref(args), *ints, _c.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(device):
+            rc = fl_ops._fn(name)(_c.byref(args), *ints, _c.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
+    fl_ops._check(rc, name)

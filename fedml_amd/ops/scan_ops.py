@@ -14,7 +14,8 @@ import ctypes as _c
 import torch
 from torch.autograd.function import once_differentiable
 
-from .fl_ops import _check, _fn, _p, _pr, _stream, use_native
+from ._launch import launch, ptr, ptr_read
+from .fl_ops import use_native
 
 _TILE = 64                # steps between two kept states
 _I32 = 2 ** 31 - 1
@@ -25,10 +26,6 @@ class _Args(_c.Structure):
                                            "agg", "mask")] + \
                [(n, _c.c_int64 * 3) for n in ("xs", "gs", "dys", "ys", "ms")] + \
                [(n, _c.c_int) for n in ("C", "T", "B", "H", "nseg", "tps")]
-
-
-def _v(p):
-    return None if p is None else p.value
 
 
 def _dense(t):
@@ -44,30 +41,28 @@ def _like(x):
     return torch.empty(C, T, B, H, dtype=x.dtype, device=x.device)
 
 
-def _launch(a, x, gate, mask, streams, bwd):
+def _run(a, x, gate, mask, streams, bwd):
     C, T, B, H = x.shape
     a.C, a.T, a.B, a.H = C, T, B, H
-    a.x, a.gate, a.mask = _v(_pr(x)), _v(_pr(gate)), _v(_pr(mask))
+    a.x, a.gate, a.mask = ptr_read(x), ptr_read(gate), ptr_read(mask)
     a.xs[:], a.gs[:] = x.stride()[:3], gate.stride()[:3]
     if mask is not None:
         a.ms[:] = mask.stride()
-    vec = 2
-    for t in (x, gate, *streams):       # two features at a time where every row starts at a multiple of two
-        if H % 2 or t.data_ptr() % (2 * t.element_size()) or any(s % 2 for s in t.stride()[:3]):
-            vec = 1
+    odd, es = H, x.element_size()           # two features at a time where every row starts at a multiple of two
+    for t in (x, gate, *streams):
+        s0, s1, s2, _ = t.stride()
+        odd |= s0 | s1 | s2 | t.data_ptr() // es
+    vec = 2 - (odd & 1)
     wgs, ntile = C * B * -(-H // (32 * vec)), -(-T // _TILE)
     nseg = 1 if wgs >= 512 else min(ntile, -(-1024 // wgs), 64)
     a.tps = -(-ntile // nseg)
-    a.nseg = -(-ntile // a.tps)
-    if wgs * a.nseg > _I32:
+    a.nseg = nseg = -(-ntile // a.tps)
+    if wgs * nseg > _I32:
         raise ValueError(f"gated_scan: {C} clients · {B} sequences · {H} features are too many for one call")
-    agg = None
-    if a.nseg > 1:
-        agg = torch.empty(C * B * a.nseg * 2 * H, dtype=torch.float32, device=x.device)
-        a.agg = _v(_p(agg))
-    with torch.cuda.device(x.device):
-        _check(_fn("fa_gated_scan")(_c.byref(a), _c.c_int(int(x.dtype == torch.bfloat16)), _c.c_int(vec),
-                                    _c.c_int(int(bwd)), _stream(x)), "fa_gated_scan")
+    if nseg > 1:
+        agg = torch.empty(C * B * nseg * 2 * H, dtype=torch.float32, device=x.device)
+        a.agg = ptr(agg)
+    launch("fa_gated_scan", a, (x.dtype == torch.bfloat16, vec, bwd), x.device)
 
 
 def _forward(x, gate, h0, mask, keep):
@@ -75,10 +70,11 @@ def _forward(x, gate, h0, mask, keep):
     y = _like(x)
     hT = torch.empty(C, B, H, dtype=torch.float32, device=x.device)
     ckpt = torch.empty(C, -(-T // _TILE), B, H, dtype=torch.float32, device=x.device) if keep else None
-    if y.numel():
-        a = _Args(y=_v(_p(y)), hT=_v(_p(hT)), h0=_v(_pr(h0)), ckpt=_v(_p(ckpt)))
+    if C * B:
+        a = _Args()
+        a.y, a.hT, a.h0, a.ckpt = ptr(y), ptr(hT), ptr_read(h0), ptr(ckpt)
         a.ys[:] = y.stride()[:3]
-        _launch(a, x, gate, mask, (y,), False)
+        _run(a, x, gate, mask, (y,), False)
     return y, hT, ckpt
 
 
@@ -102,11 +98,12 @@ class _GatedScan(torch.autograd.Function):
         dh = None if dh is None else dh.contiguous()
         dx, dgate = _like(x), _like(x)
         dh0 = torch.empty(C, B, H, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
-        if dx.numel():
-            a = _Args(dy=_v(_pr(dy)), dh=_v(_pr(dh)), dx=_v(_p(dx)), dgate=_v(_p(dgate)), dh0=_v(_p(dh0)),
-                      ckpt=_v(_pr(ckpt)))
+        if C * B:
+            a = _Args()
+            a.dy, a.dh, a.dx, a.dgate = ptr_read(dy), ptr_read(dh), ptr(dx), ptr(dgate)
+            a.dh0, a.ckpt = ptr(dh0), ptr_read(ckpt)
             a.ys[:], a.dys[:] = dx.stride()[:3], dy.stride()[:3]
-            _launch(a, x, gate, mask, (dx, dgate, dy), True)
+            _run(a, x, gate, mask, (dx, dgate, dy), True)
         return dx, dgate, dh0, None
 
 
@@ -161,7 +158,7 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, h0: torch.Tensor = None, mas
         return _scan_ref(x, gate, h0, mask)
     if mask is not None:
         mask = (mask if mask.dtype == torch.bool else mask != 0).view(torch.uint8)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, h0)):
+    if (x.requires_grad or gate.requires_grad or (h0 is not None and h0.requires_grad)) and torch.is_grad_enabled():
         return _GatedScan.apply(x, gate, h0, mask)
     y, hT, _ = _forward(_dense(x), _dense(gate), None if h0 is None else h0.contiguous(), mask, False)
     return y, hT

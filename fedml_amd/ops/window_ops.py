@@ -21,6 +21,7 @@ import math
 import torch
 from torch.autograd.function import once_differentiable
 
+from ._launch import launch, ptr, ptr_read
 from .fl_ops import _check, _fn, _i64, _p, _pr, _stream, use_native
 
 MAX_SINKS = 64
@@ -105,9 +106,9 @@ def _common(q, k, v, H, kv_heads, window, sinks):
 
 
 def _bias(bias, sequences, H, max_distance, device):
-    """The table as [C, H, buckets] and its borders."""
+    """The table as [C, H, buckets]."""
     if bias is None:
-        return None, ()
+        return None
     if bias.dim() not in (2, 3) or bias.shape[-2] != H:
         raise ValueError(f"bias: [H, buckets] or [C, H, buckets] with H = {H} expected, got {tuple(bias.shape)}")
     if bias.device != device:
@@ -119,7 +120,8 @@ def _bias(bias, sequences, H, max_distance, device):
     C = bias.shape[0]
     if C < 1 or sequences % C:
         raise ValueError(f"bias of {C} clients for {sequences} sequences")
-    return bias, relative_bucket_starts(bias.shape[-1], max_distance)
+    relative_bucket_starts(bias.shape[-1], max_distance)      # its own refusals
+    return bias
 
 
 def _scale(scale, D):
@@ -136,16 +138,6 @@ def _aligned(t):
             t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
-
-
-def _v(p):
-    return None if p is None else p.value
-
-
-def _launch(name, args, dtype, D, t):
-    bf16 = int(dtype == torch.bfloat16)
-    with torch.cuda.device(t.device):
-        _check(_fn(name)(_c.byref(args), _c.c_int(bf16), _c.c_int(D), _stream(t)), name)
 
 
 # ------------------------------------------------------------------------------------------------------- reference
@@ -183,67 +175,79 @@ def _window_ref(q, k, v, S, H, KV, W, sinks, mask, bias, max_distance, scale):
 
 
 # --------------------------------------------------------------------------------------------------------- training
-def _args(q, k, v, mask, bias, starts, cfg):
-    S, H, KV, W, sinks, D, max_distance, scale = cfg
-    a = _Args(q=_v(_pr(q)), k=_v(_pr(k)), v=_v(_pr(v)), mask=_v(_pr(mask)), bias=_v(_pr(bias)), ldq=q.stride(0),
-              ldk=k.stride(0), ldv=v.stride(0), N=q.shape[0] // S, S=S, H=H, KV=KV, C=1 if bias is None else
-              bias.shape[0], W=W, sinks=sinks, NB=len(starts), maxd=max_distance if starts else 0, scale=scale)
-    a.start[:len(starts)] = starts
+@functools.lru_cache(maxsize=256)
+def _plan(N, S, H, KV, W, sinks, scale, C, buckets, max_distance):
+    """What the kernels' arguments hold for all calls of these sizes."""
+    a = _Args(N=N, S=S, H=H, KV=KV, C=C, W=W, sinks=sinks, NB=buckets, scale=scale)
+    if buckets:
+        a.maxd = max_distance
+        a.start[:buckets] = relative_bucket_starts(buckets, max_distance)
+    if sinks and S > W:                     # the sink pass: chunks of queries about as long as a window's walk
+        a.qchunk = max(512, -(-(W + 128) // 128) * 128)
+        a.nchunk = -(-(S - W) // a.qchunk)
     return a
 
 
-def _forward(q, k, v, mask, bias, starts, cfg, keep, exact):
+def _args(q, k, v, mask, bias, cfg):
+    a = _Args.from_buffer_copy(_plan(*cfg[1:]))
+    a.q, a.k, a.v, a.mask, a.bias = ptr_read(q), ptr_read(k), ptr_read(v), ptr_read(mask), ptr_read(bias)
+    a.ldq, a.ldk, a.ldv = q.stride(0), k.stride(0), v.stride(0)
+    return a
+
+
+def _forward(q, k, v, mask, bias, cfg, keep, exact):
     """(o, o before its rounding, log-sum-exp); keep: for a backward pass, exact: with a gradient of the bias."""
-    S, H, D = cfg[0], cfg[1], cfg[5]
-    o = torch.empty(q.shape[0], H * D, dtype=q.dtype, device=q.device)
+    D, N, S, H = cfg[:4]
+    bf16, dev = q.dtype == torch.bfloat16, q.device
+    o = torch.empty(N * S, H * D, dtype=q.dtype, device=dev)
     o32 = lse = None
     if keep:
-        o32 = o if q.dtype == torch.float32 else torch.empty(o.shape, dtype=torch.float32, device=q.device)
-        lse = torch.empty(q.shape[0] // S, H, S, dtype=torch.float32, device=q.device)
-    if q.shape[0]:
-        a = _args(q, k, v, mask, bias, starts, cfg)
-        a.o, a.o32, a.lse, a.exact = _v(_p(o)), _v(_p(o32)), _v(_p(lse)), int(exact)
-        _launch("fa_window_fwd", a, q.dtype, D, q)
+        o32 = torch.empty(N * S, H * D, dtype=torch.float32, device=dev) if bf16 else o
+        lse = torch.empty(N, H, S, dtype=torch.float32, device=dev)
+    if N:
+        a = _args(q, k, v, mask, bias, cfg)
+        a.o, a.o32, a.lse, a.exact = ptr(o), ptr(o32), ptr(lse), exact
+        launch("fa_window_fwd", a, (bf16, D), dev)
     return o, o32, lse
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, bias, mask, starts, cfg):
+    def forward(ctx, q, k, v, bias, mask, cfg):
         q, k, v = _aligned(q), _aligned(k), _aligned(v)
         tab = None if bias is None else bias.contiguous()
-        o, o32, lse = _forward(q, k, v, mask, tab, starts, cfg, True, bias is not None and ctx.needs_input_grad[3])
+        o, o32, lse = _forward(q, k, v, mask, tab, cfg, True, bias is not None and ctx.needs_input_grad[3])
         ctx.save_for_backward(q, k, v, tab, mask, o32, lse)
-        ctx.starts, ctx.cfg = starts, cfg
+        ctx.cfg = cfg
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
         q, k, v, bias, mask, o32, lse = ctx.saved_tensors
-        S, H, KV, W, sinks, D, _, _ = ctx.cfg
-        N, dev = q.shape[0] // S, q.device
-        do = _aligned(do.to(q.dtype))
-        dq = torch.empty(N * S, H * D, dtype=q.dtype, device=dev)
-        dk = torch.empty(N * S, KV * D, dtype=q.dtype, device=dev)
-        dv = torch.empty_like(dk)
-        dbias = torch.zeros_like(bias) if bias is not None and ctx.needs_input_grad[3] else None
+        D, N, S, H, KV = ctx.cfg[:5]
+        dev, dt, f32 = q.device, q.dtype, torch.float32
+        do = _aligned(do if do.dtype == dt else do.to(dt))
+        dq = torch.empty(N * S, H * D, dtype=dt, device=dev)
+        dk = torch.empty(N * S, KV * D, dtype=dt, device=dev)
+        dv = torch.empty(N * S, KV * D, dtype=dt, device=dev)
+        dbias = None
+        if bias is not None and ctx.needs_input_grad[3]:
+            dbias = torch.empty(bias.shape, dtype=f32, device=dev) if N else torch.zeros_like(bias)
         if N:
-            a = _args(q, k, v, mask, bias, ctx.starts, ctx.cfg)
-            tile = 128 if S > 64 else 32                  # queries of a workgroup of the dq kernel
-            dsum = torch.empty(N, H, S, dtype=torch.float32, device=dev)
+            a = _args(q, k, v, mask, bias, ctx.cfg)
+            dsum = torch.empty(N, H, S, dtype=f32, device=dev)
             part = bpart = None
-            if sinks and S > W:
-                a.qchunk = max(512, -(-(W + 128) // 128) * 128)
-                a.nchunk = -(-(S - W) // a.qchunk)
-                part = torch.empty(N, KV, a.nchunk + 1, 2, sinks, D, dtype=torch.float32, device=dev)
+            if a.nchunk:
+                part = torch.empty(N, KV, a.nchunk + 1, 2, a.sinks, D, dtype=f32, device=dev)
             if dbias is not None:
-                bpart = torch.empty(N, H, -(-S // tile), bias.shape[-1], dtype=torch.float32, device=dev)
-            a.dout, a.lddo, a.lse, a.o32 = _v(_pr(do)), do.stride(0), _v(_pr(lse)), _v(_pr(o32))
-            a.dq, a.dk, a.dv, a.dsum = _v(_p(dq)), _v(_p(dk)), _v(_p(dv)), _v(_p(dsum))
-            a.part, a.bpart, a.dbias = _v(_p(part)), _v(_p(bpart)), _v(_p(dbias))
-            _launch("fa_window_bwd", a, q.dtype, D, q)
-        return dq, dk, dv, dbias, None, None, None
+                tile = 128 if S > 64 else 32                  # queries of a workgroup of the dq kernel
+                bpart = torch.empty(N, H, -(-S // tile), bias.shape[-1], dtype=f32, device=dev)
+            a.dout, a.lddo, a.lse, a.o32 = ptr_read(do), do.stride(0), ptr_read(lse), ptr_read(o32)
+            a.dq, a.dk, a.dv, a.dsum = ptr(dq), ptr(dk), ptr(dv), ptr(dsum)
+            a.part, a.bpart, a.dbias = ptr(part), ptr(bpart), ptr(dbias)
+            launch("fa_window_bwd", a, (dt == torch.bfloat16, D), dev)
+        return dq, dk, dv, dbias, None, None
 
 
 def window_attention(q, k, v, S: int, H: int, window: int, sinks: int = 0, kv_heads: int = None,
@@ -270,17 +274,19 @@ def window_attention(q, k, v, S: int, H: int, window: int, sinks: int = 0, kv_he
         if mask.shape != (N, S) or mask.dtype.is_floating_point or mask.dtype.is_complex or mask.device != q.device:
             raise ValueError(f"mask: bool or integer [{N}, {S}] on {q.device} expected, got {mask.dtype} "
                              f"{tuple(mask.shape)} on {mask.device}")
-    table, starts = _bias(bias, N, H, max_distance, q.device)
+    table = _bias(bias, N, H, max_distance, q.device)
     scale = _scale(scale, D)
     if not use_native(q):
         return _window_ref(q, k, v, S, H, KV, W, sinks, mask, table, max_distance, scale)
     if mask is not None:
         mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous().view(torch.uint8)
-    cfg = (S, H, KV, min(W, S), min(sinks, S), D, int(max_distance), scale)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table)):
-        return _WindowAttention.apply(q, k, v, table, mask, starts, cfg)
+    cfg = (D, N, S, H, KV, min(W, S), min(sinks, S), scale, *((0, 0, 0) if table is None else
+                                                              (table.shape[0], table.shape[2], int(max_distance))))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                    (table is not None and table.requires_grad)):
+        return _WindowAttention.apply(q, k, v, table, mask, cfg)
     tab = None if table is None else table.contiguous()
-    return _forward(_aligned(q), _aligned(k), _aligned(v), mask, tab, starts, cfg, False, False)[0]
+    return _forward(_aligned(q), _aligned(k), _aligned(v), mask, tab, cfg, False, False)[0]
 
 
 # ---------------------------------------------------------------------------------------------------------- serving
@@ -331,6 +337,23 @@ def _step_ref(q, k, v, kc, vc, pos, H, KV, W, sinks, bias, max_distance, scale):
     return (w.unsqueeze(2) @ vh).reshape(B, H * D).to(q.dtype)
 
 
+@functools.lru_cache(maxsize=256)
+def _step_plan(B, H, KV, W, sinks, scale, C, buckets, max_distance):
+    # enough workgroups for 256 CUs, of at least one 32-slot tile a wave
+    n, wgs = W + sinks, B * KV * -(-(H // KV) // 32)
+    tiles = -(-n // 128)
+    splits = max(1, min(tiles, -(-512 // wgs)))
+    per = -(-tiles // splits) * 128
+    splits = -(-n // per)
+    if wgs * splits > _I32 or B * H > _I32 or n > 2 ** 30:
+        raise ValueError(f"{B} sequences of {H} heads and {n} slots are too many for one call")
+    a = _StepArgs(B=B, H=H, KV=KV, C=C, W=W, sinks=sinks, NB=buckets, splits=splits, per=per, scale=scale)
+    if buckets:
+        a.maxd = max_distance
+        a.start[:buckets] = relative_bucket_starts(buckets, max_distance)
+    return a
+
+
 def window_attention_step(q, k, v, k_cache, v_cache, pos, H: int, window: int, sinks: int = 0, kv_heads: int = None,
                           bias: torch.Tensor = None, max_distance: int = 128, scale: float = None):
     """:func:`window_attention` of one new token per sequence: ``q`` [B, H·D], ``k`` / ``v`` [B, kv_heads·D] are its
@@ -343,9 +366,10 @@ def window_attention_step(q, k, v, k_cache, v_cache, pos, H: int, window: int, s
     B, n = q.shape[0], W + sinks
     _cache(k_cache, v_cache, B, KV, D, n, q.dtype, q.device)
     pos = _pos(pos, B, q.device, "pos")
-    table, starts = _bias(bias, B, H, max_distance, q.device)
+    table = _bias(bias, B, H, max_distance, q.device)
     scale = _scale(scale, D)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
+    if (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)) and \
+            torch.is_grad_enabled():
         raise ValueError("window_attention_step computes no gradient: call it under torch.no_grad()")
     if not use_native(q):
         return _step_ref(q, k, v, k_cache, v_cache, pos, H, KV, W, sinks, table, max_distance, scale)
@@ -354,23 +378,17 @@ def window_attention_step(q, k, v, k_cache, v_cache, pos, H: int, window: int, s
         return o
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
     tab = None if table is None else table.contiguous()
-    # enough workgroups for 256 CUs, of at least one 32-slot tile a wave
-    wgs = B * KV * -(-(H // KV) // 32)
-    tiles = -(-n // 128)
-    splits = max(1, min(tiles, -(-512 // wgs)))
-    per = -(-tiles // splits) * 128
-    splits = -(-n // per)
-    if wgs * splits > _I32 or B * H > _I32:
-        raise ValueError(f"{B} sequences of {H} heads are too many for one call")
-    a = _StepArgs(q=_v(_pr(q)), k=_v(_pr(k)), v=_v(_pr(v)), kc=_v(_p(k_cache)), vc=_v(_p(v_cache)), o=_v(_p(o)),
-                  pos=_v(_pr(pos)), bias=_v(_pr(tab)), ldq=q.stride(0), ldk=k.stride(0), ldv=v.stride(0), B=B, H=H,
-                  KV=KV, C=1 if tab is None else tab.shape[0], W=W, sinks=sinks, NB=len(starts),
-                  maxd=int(max_distance) if starts else 0, splits=splits, per=per, scale=scale)
-    a.start[:len(starts)] = starts
-    if splits > 1:
-        part = torch.empty(B * H * splits * (D + 2), dtype=torch.float32, device=q.device)
-        a.pacc, a.pml = _v(_p(part)), _v(_p(part[B * H * splits * D:]))
-    _launch("fa_window_step", a, q.dtype, D, q)
+    plan = _step_plan(B, H, KV, W, sinks, scale, *((1, 0, 0) if tab is None else
+                                                   (tab.shape[0], tab.shape[2], int(max_distance))))
+    a = _StepArgs.from_buffer_copy(plan)
+    a.q, a.k, a.v, a.kc, a.vc = ptr_read(q), ptr_read(k), ptr_read(v), ptr(k_cache), ptr(v_cache)
+    a.o, a.pos, a.bias = ptr(o), ptr_read(pos), ptr_read(tab)
+    a.ldq, a.ldk, a.ldv = q.stride(0), k.stride(0), v.stride(0)
+    if a.splits > 1:
+        part = torch.empty(B * H * a.splits * (D + 2), dtype=torch.float32, device=q.device)
+        a.pacc = ptr(part)
+        a.pml = a.pacc + 4 * B * H * a.splits * D
+    launch("fa_window_step", a, (q.dtype == torch.bfloat16, D), q.device)
     return o
 
 

@@ -5,9 +5,9 @@
 // A masked step has f = 1 and takes nothing: the state passes it, y, dx and dgate are zero there.
 //
 // Any run of steps is an affine map of the state, h → A h + B, and maps compose: a workgroup owns 32·V features of one
-// sequence and walks the time in tiles of 64 steps; 8 groups of 32 lanes take 8 steps each in registers, put their maps
+// sequence and walks the time in tiles of 32 steps; 8 groups of 32 lanes take 4 steps each in registers, put their maps
 // into LDS, and every group composes those before it. The carried state stays in fp32 registers; x and gate are read
-// once. The forward leaves the state before every tile (fp32, 1/64 of the states): the backward recomputes the
+// once. The forward leaves the state before every tile (fp32, 1/32 of the states): the backward recomputes the
 // others in registers from there, so it reads x, gate and dy only and loses nothing to the rounding of y.
 // Few features and a long time: the time is cut into segments, whose maps a first kernel forms (same reads); the
 // workgroups of the second compose those before (after, backward) their segment. Order fixed, no atomics.
@@ -15,7 +15,7 @@
 
 namespace scan {
 
-constexpr int kTile = 64, kGroups = 8, kSteps = kTile / kGroups;
+constexpr int kTile = 32, kGroups = 8, kSteps = kTile / kGroups;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
@@ -25,7 +25,7 @@ struct Args {
   float *hT, *dh0, *ckpt, *agg;
   const uint8_t* mask;
   int64_t xs[3], gs[3], dys[3], ys[3], ms[3];   // element strides over client, time and sequence; y, dx and dgate share ys
-  int C, T, B, H, nseg, tps;                    // tps: tiles of a segment
+  int C, T, B, H, nseg, tps;                    // tps: tiles of a segment, even if there are several
 };
 
 template <typename T, int V> struct Vec;
@@ -69,58 +69,76 @@ __device__ __forceinline__ void gates(float g, float& f, float& keep) {
 
 // where a workgroup and a thread stand
 template <int V> struct At {
-  int c, b, seg, lane, grp, j;
+  int c, b, seg, lane, grp, j, jr;       // jr: a feature that exists
   bool on;
   __device__ __forceinline__ explicit At(const Args& a) {
     const int nft = (a.H + 32 * V - 1) / (32 * V);
-    int64_t id = blockIdx.x;
-    const int ft = (int)(id % nft);
+    // consecutive work items to the same XCD (workgroup ids go round the 8 of them): where rows are no whole cache
+    // lines, the two workgroups that share one meet in one L2
+    const int per = gridDim.x >> 3, wg = blockIdx.x;
+    int id = wg < per * 8 ? (wg & 7) * per + (wg >> 3) : wg;
+    const int ft = id % nft;
     id /= nft;
-    seg = (int)(id % a.nseg);
+    seg = id % a.nseg;
     id /= a.nseg;
-    b = (int)(id % a.B);
-    c = (int)(id / a.B);
+    b = id % a.B;
+    c = id / a.B;
     lane = threadIdx.x & 31;
     grp = threadIdx.x >> 5;
     j = (ft * 32 + lane) * V;
     on = j < a.H;
+    jr = on ? j : 0;
   }
 };
 
-// one stream of a thread's 8 steps of a tile
-template <typename T, int V> struct Steps {
-  typename Vec<T, V>::raw r[kSteps];
-  __device__ __forceinline__ void load(const T* p, int64_t st, int t0, int T_, bool on) {
+// one stream of a thread's N steps; every load is made, of steps up to the last and features that exist
+template <typename T, int V, int N> struct Steps {
+  typename Vec<T, V>::raw r[N];
+  __device__ __forceinline__ void load(const T* p, int64_t st, int t0, int T_) {
+    if (t0 + N <= T_) {
+      const T* q = p + t0 * st;
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      r[i] = typename Vec<T, V>::raw{};
-      if (on && t0 + i < T_) r[i] = *reinterpret_cast<const typename Vec<T, V>::raw*>(p + (t0 + i) * st);
+      for (int i = 0; i < N; ++i, q += st) r[i] = *reinterpret_cast<const typename Vec<T, V>::raw*>(q);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        r[i] = *reinterpret_cast<const typename Vec<T, V>::raw*>(p + (t0 + i < T_ ? t0 + i : T_ - 1) * st);
     }
   }
 };
 
-// bit i: step t0 + i exists and is no padding
-__device__ __forceinline__ uint32_t real_steps(const uint8_t* m, int64_t st, int t0, int T_) {
-  uint32_t bits = 0;
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i)
-    if (t0 + i < T_ && (!m || m[(t0 + i) * st])) bits |= 1u << i;
-  return bits;
+// lane i < N of a group: is step t0 + i one of the text's
+template <int N> __device__ __forceinline__ int real_step(const uint8_t* m, int64_t st, int t0, int T_, int lane) {
+  const int t = t0 + (lane & (N - 1));
+  const int r = m ? m[(t < T_ ? t : T_ - 1) * st] : 1;
+  return t < T_ ? r : 0;
+}
+// bit i: step t0 + i of this thread's group
+template <int N> __device__ __forceinline__ uint32_t real_bits(int real) {
+  return (uint32_t)((uint64_t)__ballot(real != 0) >> (threadIdx.x & 32)) & ((1u << N) - 1);
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void step_values(const Steps<T, V>& x, const Steps<T, V>& g, uint32_t bits, int i, float* f,
-                                            float* keep, float* xv) {
-  float gv[V];
-  Vec<T, V>::get(g.r[i], gv);
-  Vec<T, V>::get(x.r[i], xv);
-  const bool real = (bits >> i) & 1;
+template <typename T, int V, int N>
+__device__ __forceinline__ void values(const Steps<T, V, N>& x, const Steps<T, V, N>& g, uint32_t bits, float (*f)[V],
+                                       float (*keep)[V], float (*xv)[V]) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    gates(gv[v], f[v], keep[v]);
-    f[v] = real ? f[v] : 1.f;
-    keep[v] = real ? keep[v] : 0.f;
-    xv[v] = real ? xv[v] : 0.f;
+  for (int i = 0; i < N; ++i) {
+    float gv[V];
+    Vec<T, V>::get(g.r[i], gv);
+    Vec<T, V>::get(x.r[i], xv[i]);
+#pragma unroll
+    for (int v = 0; v < V; ++v) gates(gv[v], f[i][v], keep[i][v]);
+  }
+  if (__any(bits != (1u << N) - 1)) {      // padding somewhere: a step of it keeps the state and takes nothing
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const bool real = (bits >> i) & 1;
+        f[i][v] = real ? f[i][v] : 1.f;
+        keep[i][v] = real ? keep[i][v] : 0.f;
+        xv[i][v] = real ? xv[i][v] : 0.f;
+      }
   }
 }
 
@@ -129,8 +147,8 @@ template <typename T, int V> __global__ __launch_bounds__(256) void fwd_kernel(c
   const At<V> at(a);
   const int ntile = (a.T + kTile - 1) / kTile;
   const int k0 = at.seg * a.tps, k1 = k0 + a.tps < ntile ? k0 + a.tps : ntile;
-  const T* x = (const T*)a.x + at.c * a.xs[0] + at.b * a.xs[2] + at.j;
-  const T* g = (const T*)a.gate + at.c * a.gs[0] + at.b * a.gs[2] + at.j;
+  const T* x = (const T*)a.x + at.c * a.xs[0] + at.b * a.xs[2] + at.jr;
+  const T* g = (const T*)a.gate + at.c * a.gs[0] + at.b * a.gs[2] + at.jr;
   T* y = (T*)a.y + at.c * a.ys[0] + at.b * a.ys[2] + at.j;
   const uint8_t* m = a.mask ? a.mask + at.c * a.ms[0] + at.b * a.ms[2] : nullptr;
   const int64_t chan = ((int64_t)at.c * a.B + at.b) * a.H + at.j;
@@ -142,13 +160,20 @@ template <typename T, int V> __global__ __launch_bounds__(256) void fwd_kernel(c
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = fmaf(p[v], h[v], p[a.H + v]);
   }
-  Steps<T, V> rx, rg;
-  uint32_t bits = real_steps(m, a.ms[1], k0 * kTile + at.grp * kSteps, a.T);
-  rx.load(x, a.xs[1], k0 * kTile + at.grp * kSteps, a.T, at.on);
-  rg.load(g, a.gs[1], k0 * kTile + at.grp * kSteps, a.T, at.on);
+  Steps<T, V, kSteps> rx, rg;
+  int real;
+  auto load = [&](int k) {
+    const int t0 = k * kTile + at.grp * kSteps;
+    real = real_step<kSteps>(m, a.ms[1], t0, a.T, at.lane);
+    rx.load(x, a.xs[1], t0, a.T);
+    rg.load(g, a.gs[1], t0, a.T);
+  };
+  load(k0);
   for (int k = k0; k < k1; ++k) {
     const int t0 = k * kTile + at.grp * kSteps, buf = k & 1;
-    float f[kSteps][V], in[kSteps][V], A[V], Bv[V];
+    const uint32_t bits = real_bits<kSteps>(real);
+    float f[kSteps][V], keep[kSteps][V], in[kSteps][V], A[V], Bv[V];
+    values<T, V, kSteps>(rx, rg, bits, f, keep, in);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       A[v] = 1.f;
@@ -156,11 +181,9 @@ template <typename T, int V> __global__ __launch_bounds__(256) void fwd_kernel(c
     }
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      float keep[V], xv[V];
-      step_values<T, V>(rx, rg, bits, i, f[i], keep, xv);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        in[i][v] = keep[v] * xv[v];
+        in[i][v] *= keep[i][v];
         A[v] *= f[i][v];
         Bv[v] = fmaf(f[i][v], Bv[v], in[i][v]);
       }
@@ -170,12 +193,7 @@ template <typename T, int V> __global__ __launch_bounds__(256) void fwd_kernel(c
       sA[buf][at.grp][at.lane * V + v] = A[v];
       sB[buf][at.grp][at.lane * V + v] = Bv[v];
     }
-    const uint32_t now = bits;
-    if (k + 1 < k1) {
-      bits = real_steps(m, a.ms[1], t0 + kTile, a.T);
-      rx.load(x, a.xs[1], t0 + kTile, a.T, at.on);
-      rg.load(g, a.gs[1], t0 + kTile, a.T, at.on);
-    }
+    if (k + 1 < k1) load(k + 1);
     if (a.ckpt && at.grp == 0 && at.on) {
       float* p = a.ckpt + (((int64_t)at.c * ntile + k) * a.B + at.b) * a.H + at.j;
 #pragma unroll
@@ -196,7 +214,7 @@ template <typename T, int V> __global__ __launch_bounds__(256) void fwd_kernel(c
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         s[v] = fmaf(f[i][v], s[v], in[i][v]);
-        o[v] = (now >> i) & 1 ? s[v] : 0.f;
+        o[v] = (bits >> i) & 1 ? s[v] : 0.f;
       }
       if (at.on && t0 + i < a.T)
         *reinterpret_cast<typename Vec<T, V>::raw*>(y + (t0 + i) * a.ys[1]) = Vec<T, V>::put(o);
@@ -212,9 +230,9 @@ template <typename T, int V> __global__ __launch_bounds__(256) void bwd_kernel(c
   const At<V> at(a);
   const int ntile = (a.T + kTile - 1) / kTile;
   const int k0 = at.seg * a.tps, k1 = k0 + a.tps < ntile ? k0 + a.tps : ntile;
-  const T* x = (const T*)a.x + at.c * a.xs[0] + at.b * a.xs[2] + at.j;
-  const T* g = (const T*)a.gate + at.c * a.gs[0] + at.b * a.gs[2] + at.j;
-  const T* dy = (const T*)a.dy + at.c * a.dys[0] + at.b * a.dys[2] + at.j;
+  const T* x = (const T*)a.x + at.c * a.xs[0] + at.b * a.xs[2] + at.jr;
+  const T* g = (const T*)a.gate + at.c * a.gs[0] + at.b * a.gs[2] + at.jr;
+  const T* dy = (const T*)a.dy + at.c * a.dys[0] + at.b * a.dys[2] + at.jr;
   T* dx = (T*)a.dx + at.c * a.ys[0] + at.b * a.ys[2] + at.j;
   T* dg = (T*)a.dgate + at.c * a.ys[0] + at.b * a.ys[2] + at.j;
   const uint8_t* m = a.mask ? a.mask + at.c * a.ms[0] + at.b * a.ms[2] : nullptr;
@@ -227,23 +245,25 @@ template <typename T, int V> __global__ __launch_bounds__(256) void bwd_kernel(c
 #pragma unroll
     for (int v = 0; v < V; ++v) G[v] = fmaf(p[v], G[v], p[a.H + v]);
   }
-  Steps<T, V> rx, rg, rd;
+  Steps<T, V, kSteps> rx, rg, rd;
   float hn[V];                                               // the state before the tile
-  uint32_t bits;
+  int real;
   auto load = [&](int k) {
     const int t0 = k * kTile + at.grp * kSteps;
-    bits = real_steps(m, a.ms[1], t0, a.T);
-    rx.load(x, a.xs[1], t0, a.T, at.on);
-    rg.load(g, a.gs[1], t0, a.T, at.on);
-    rd.load(dy, a.dys[1], t0, a.T, at.on);
-    const float* p = a.ckpt + (((int64_t)at.c * ntile + k) * a.B + at.b) * a.H + at.j;
+    real = real_step<kSteps>(m, a.ms[1], t0, a.T, at.lane);
+    rx.load(x, a.xs[1], t0, a.T);
+    rg.load(g, a.gs[1], t0, a.T);
+    rd.load(dy, a.dys[1], t0, a.T);
+    const float* p = a.ckpt + (((int64_t)at.c * ntile + k) * a.B + at.b) * a.H + at.jr;
 #pragma unroll
-    for (int v = 0; v < V; ++v) hn[v] = at.on ? p[v] : 0.f;
+    for (int v = 0; v < V; ++v) hn[v] = p[v];
   };
   load(k1 - 1);
   for (int k = k1 - 1; k >= k0; --k) {
     const int t0 = k * kTile + at.grp * kSteps, buf = k & 1;
+    const uint32_t bits = real_bits<kSteps>(real);
     float f[kSteps][V], keep[kSteps][V], xv[kSteps][V], d[kSteps][V], A[V], Bv[V], Gv[V];
+    values<T, V, kSteps>(rx, rg, bits, f, keep, xv);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       A[v] = 1.f;
@@ -251,7 +271,6 @@ template <typename T, int V> __global__ __launch_bounds__(256) void bwd_kernel(c
     }
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      step_values<T, V>(rx, rg, bits, i, f[i], keep[i], xv[i]);
       Vec<T, V>::get(rd.r[i], d[i]);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
@@ -325,13 +344,14 @@ template <typename T, int V, bool BWD> __global__ __launch_bounds__(256) void ag
   const At<V> at(a);
   const int ntile = (a.T + kTile - 1) / kTile;
   const int k0 = at.seg * a.tps, k1 = k0 + a.tps < ntile ? k0 + a.tps : ntile;
-  const T* g = (const T*)a.gate + at.c * a.gs[0] + at.b * a.gs[2] + at.j;
-  const T* o = BWD ? (const T*)a.dy + at.c * a.dys[0] + at.b * a.dys[2] + at.j
-                   : (const T*)a.x + at.c * a.xs[0] + at.b * a.xs[2] + at.j;
+  const T* g = (const T*)a.gate + at.c * a.gs[0] + at.b * a.gs[2] + at.jr;
+  const T* o = BWD ? (const T*)a.dy + at.c * a.dys[0] + at.b * a.dys[2] + at.jr
+                   : (const T*)a.x + at.c * a.xs[0] + at.b * a.xs[2] + at.jr;
   const int64_t ot = BWD ? a.dys[1] : a.xs[1];
   const uint8_t* m = a.mask ? a.mask + at.c * a.ms[0] + at.b * a.ms[2] : nullptr;
   // a group walks a run of the segment of its own: its map is formed without a barrier
-  const int run = ((k1 - k0) * kTile + kGroups - 1) / kGroups;       // a multiple of 8: a tile is 8 groups of 8 steps
+  constexpr int N = 8;
+  const int run = ((k1 - k0) * kTile / kGroups + N - 1) / N * N;     // whole tiles of it but in the last segment
   const int ta = k0 * kTile + at.grp * run, tb = ta + run;
   float A[V], Bv[V];
 #pragma unroll
@@ -339,29 +359,27 @@ template <typename T, int V, bool BWD> __global__ __launch_bounds__(256) void ag
     A[v] = 1.f;
     Bv[v] = 0.f;
   }
-  Steps<T, V> rg, ro;
-  uint32_t bits;
-  const int n = run / kSteps;
+  Steps<T, V, N> rg, ro;
+  int real;
+  const int n = run / N;
   auto load = [&](int i) {
-    const int t0 = BWD ? tb - (i + 1) * kSteps : ta + i * kSteps;
-    bits = real_steps(m, a.ms[1], t0, a.T);
-    rg.load(g, a.gs[1], t0, a.T, at.on);
-    ro.load(o, ot, t0, a.T, at.on);
+    const int t0 = BWD ? tb - (i + 1) * N : ta + i * N;
+    real = real_step<N>(m, a.ms[1], t0, a.T, at.lane);
+    rg.load(g, a.gs[1], t0, a.T);
+    ro.load(o, ot, t0, a.T);
   };
   load(0);
   for (int i = 0; i < n; ++i) {
-    const Steps<T, V> cg = rg, co = ro;
-    const uint32_t now = bits;
+    float f[N][V], keep[N][V], ov[N][V];
+    values<T, V, N>(ro, rg, real_bits<N>(real), f, keep, ov);
     if (i + 1 < n) load(i + 1);
 #pragma unroll
-    for (int u = 0; u < kSteps; ++u) {
-      const int r = BWD ? kSteps - 1 - u : u;
-      float f[V], keep[V], ov[V];
-      step_values<T, V>(co, cg, now, r, f, keep, ov);
+    for (int u = 0; u < N; ++u) {
+      const int r = BWD ? N - 1 - u : u;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        A[v] *= f[v];
-        Bv[v] = BWD ? f[v] * (ov[v] + Bv[v]) : fmaf(f[v], Bv[v], keep[v] * ov[v]);
+        A[v] *= f[r][v];
+        Bv[v] = BWD ? f[r][v] * (ov[r][v] + Bv[v]) : fmaf(f[r][v], Bv[v], keep[r][v] * ov[r][v]);
       }
     }
   }

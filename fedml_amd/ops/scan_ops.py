@@ -17,7 +17,7 @@ from torch.autograd.function import once_differentiable
 from ._launch import launch, ptr, ptr_read
 from .fl_ops import use_native
 
-_TILE = 64                # steps between two kept states
+_TILE = 32                # steps between two kept states
 _I32 = 2 ** 31 - 1
 
 
@@ -55,7 +55,7 @@ def _run(a, x, gate, mask, streams, bwd):
     vec = 2 - (odd & 1)
     wgs, ntile = C * B * -(-H // (32 * vec)), -(-T // _TILE)
     nseg = 1 if wgs >= 512 else min(ntile, -(-1024 // wgs), 64)
-    a.tps = -(-ntile // nseg)
+    a.tps = -(-ntile // (2 * nseg)) * 2        # pairs of tiles
     a.nseg = nseg = -(-ntile // a.tps)
     if wgs * nseg > _I32:
         raise ValueError(f"gated_scan: {C} clients · {B} sequences · {H} features are too many for one call")

@@ -69,7 +69,7 @@ __device__ __forceinline__ void gates(float g, float& f, float& keep) {
 
 // where a workgroup and a thread stand
 template <int V> struct At {
-  int c, b, seg, lane, grp, j, jr;       // jr: a feature that exists
+  int c, b, seg, lane, grp, j0, j, jr;   // features: the workgroup's first, the thread's, one that exists
   bool on;
   __device__ __forceinline__ explicit At(const Args& a) {
     const int nft = (a.H + 32 * V - 1) / (32 * V);
@@ -85,7 +85,8 @@ template <int V> struct At {
     c = id / a.B;
     lane = threadIdx.x & 31;
     grp = threadIdx.x >> 5;
-    j = (ft * 32 + lane) * V;
+    j0 = ft * 32 * V;
+    j = j0 + lane * V;
     on = j < a.H;
     jr = on ? j : 0;
   }
@@ -142,8 +143,11 @@ __device__ __forceinline__ void values(const Steps<T, V, N>& x, const Steps<T, V
   }
 }
 
+// The first 32·V threads carry the states of the workgroup's features, one each, from group to group and tile to tile
+// (the last ones, in the backward, the gradients that go the other way); a group gets what it starts from through LDS.
+// With every thread composing the maps before its own, the maps' reads cost the backward half its waves: SCAN_NOTE
 template <typename T, int V> __global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
-  __shared__ float sA[2][kGroups][32 * V], sB[2][kGroups][32 * V];
+  __shared__ float sA[kGroups][32 * V], sB[kGroups][32 * V], sS[kGroups][32 * V];
   const At<V> at(a);
   const int ntile = (a.T + kTile - 1) / kTile;
   const int k0 = at.seg * a.tps, k1 = k0 + a.tps < ntile ? k0 + a.tps : ntile;
@@ -151,14 +155,13 @@ template <typename T, int V> __global__ __launch_bounds__(256) void fwd_kernel(c
   const T* g = (const T*)a.gate + at.c * a.gs[0] + at.b * a.gs[2] + at.jr;
   T* y = (T*)a.y + at.c * a.ys[0] + at.b * a.ys[2] + at.j;
   const uint8_t* m = a.mask ? a.mask + at.c * a.ms[0] + at.b * a.ms[2] : nullptr;
-  const int64_t chan = ((int64_t)at.c * a.B + at.b) * a.H + at.j;
-  float h[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = at.on && a.h0 ? a.h0[chan + v] : 0.f;
-  for (int s = 0; s < at.seg && at.on; ++s) {      // the segments before this one
-    const float* p = a.agg + (((int64_t)at.c * a.B + at.b) * a.nseg + s) * 2 * a.H + at.j;
-#pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = fmaf(p[v], h[v], p[a.H + v]);
+  const int q = threadIdx.x, jq = at.j0 + q;           // a carrying thread's feature
+  const bool carries = q < 32 * V, onq = carries && jq < a.H;
+  const int64_t seq = (int64_t)at.c * a.B + at.b;
+  float h = onq && a.h0 ? a.h0[seq * a.H + jq] : 0.f;
+  for (int s = 0; s < at.seg && onq; ++s) {            // the segments before this one
+    const float* p = a.agg + (seq * a.nseg + s) * 2 * a.H + jq;
+    h = fmaf(p[0], h, p[a.H]);
   }
   Steps<T, V, kSteps> rx, rg;
   int real;
@@ -170,44 +173,37 @@ template <typename T, int V> __global__ __launch_bounds__(256) void fwd_kernel(c
   };
   load(k0);
   for (int k = k0; k < k1; ++k) {
-    const int t0 = k * kTile + at.grp * kSteps, buf = k & 1;
+    const int t0 = k * kTile + at.grp * kSteps;
     const uint32_t bits = real_bits<kSteps>(real);
     float f[kSteps][V], keep[kSteps][V], in[kSteps][V], A[V], Bv[V];
     values<T, V, kSteps>(rx, rg, bits, f, keep, in);
+    if (k + 1 < k1) load(k + 1);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       A[v] = 1.f;
       Bv[v] = 0.f;
-    }
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
+      for (int i = 0; i < kSteps; ++i) {
         in[i][v] *= keep[i][v];
         A[v] *= f[i][v];
         Bv[v] = fmaf(f[i][v], Bv[v], in[i][v]);
       }
+      sA[at.grp][at.lane * V + v] = A[v];
+      sB[at.grp][at.lane * V + v] = Bv[v];
     }
+    __syncthreads();
+    if (carries) {
+      if (onq && a.ckpt) a.ckpt[(((int64_t)at.c * ntile + k) * a.B + at.b) * a.H + jq] = h;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      sA[buf][at.grp][at.lane * V + v] = A[v];
-      sB[buf][at.grp][at.lane * V + v] = Bv[v];
-    }
-    if (k + 1 < k1) load(k + 1);
-    if (a.ckpt && at.grp == 0 && at.on) {
-      float* p = a.ckpt + (((int64_t)at.c * ntile + k) * a.B + at.b) * a.H + at.j;
-#pragma unroll
-      for (int v = 0; v < V; ++v) p[v] = h[v];
+      for (int i = 0; i < kGroups; ++i) {
+        sS[i][q] = h;
+        h = fmaf(sA[i][q], h, sB[i][q]);
+      }
     }
     __syncthreads();
     float s[V];
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (i == at.grp) s[v] = h[v];
-        h[v] = fmaf(sA[buf][i][at.lane * V + v], h[v], sB[buf][i][at.lane * V + v]);
-      }
+    for (int v = 0; v < V; ++v) s[v] = sS[at.grp][at.lane * V + v];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       float o[V];
@@ -220,13 +216,12 @@ template <typename T, int V> __global__ __launch_bounds__(256) void fwd_kernel(c
         *reinterpret_cast<typename Vec<T, V>::raw*>(y + (t0 + i) * a.ys[1]) = Vec<T, V>::put(o);
     }
   }
-  if (at.on && at.grp == 0 && k1 == ntile)
-#pragma unroll
-    for (int v = 0; v < V; ++v) a.hT[chan + v] = h[v];
+  if (onq && k1 == ntile) a.hT[seq * a.H + jq] = h;
 }
 
 template <typename T, int V> __global__ __launch_bounds__(256) void bwd_kernel(const Args a) {
-  __shared__ float sA[2][kGroups][32 * V], sB[2][kGroups][32 * V], sG[2][kGroups][32 * V];
+  __shared__ float sA[kGroups][32 * V], sB[kGroups][32 * V], sG[kGroups][32 * V], sS[kGroups][32 * V],
+      sE[kGroups][32 * V];
   const At<V> at(a);
   const int ntile = (a.T + kTile - 1) / kTile;
   const int k0 = at.seg * a.tps, k1 = k0 + a.tps < ntile ? k0 + a.tps : ntile;
@@ -236,17 +231,20 @@ template <typename T, int V> __global__ __launch_bounds__(256) void bwd_kernel(c
   T* dx = (T*)a.dx + at.c * a.ys[0] + at.b * a.ys[2] + at.j;
   T* dg = (T*)a.dgate + at.c * a.ys[0] + at.b * a.ys[2] + at.j;
   const uint8_t* m = a.mask ? a.mask + at.c * a.ms[0] + at.b * a.ms[2] : nullptr;
-  const int64_t chan = ((int64_t)at.c * a.B + at.b) * a.H + at.j;
-  float G[V], h[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) G[v] = at.on && a.dh ? a.dh[chan + v] : 0.f;
-  for (int s = a.nseg - 1; s > at.seg && at.on; --s) {      // the segments after this one
-    const float* p = a.agg + (((int64_t)at.c * a.B + at.b) * a.nseg + s) * 2 * a.H + at.j;
-#pragma unroll
-    for (int v = 0; v < V; ++v) G[v] = fmaf(p[v], G[v], p[a.H + v]);
+  // the first threads carry states, the last ones gradients
+  const bool fore = threadIdx.x < 32 * V, aft = threadIdx.x >= 256 - 32 * V;
+  const int q = fore ? threadIdx.x : threadIdx.x - (256 - 32 * V), jq = at.j0 + q;
+  const bool onq = (fore || aft) && jq < a.H;
+  const int64_t seq = (int64_t)at.c * a.B + at.b;
+  float G = 0.f, hn = 0.f;
+  if (aft && onq) {
+    if (a.dh) G = a.dh[seq * a.H + jq];
+    for (int s = a.nseg - 1; s > at.seg; --s) {              // the segments after this one
+      const float* p = a.agg + (seq * a.nseg + s) * 2 * a.H + jq;
+      G = fmaf(p[0], G, p[a.H]);
+    }
   }
   Steps<T, V, kSteps> rx, rg, rd;
-  float hn[V];                                               // the state before the tile
   int real;
   auto load = [&](int k) {
     const int t0 = k * kTile + at.grp * kSteps;
@@ -254,69 +252,65 @@ template <typename T, int V> __global__ __launch_bounds__(256) void bwd_kernel(c
     rx.load(x, a.xs[1], t0, a.T);
     rg.load(g, a.gs[1], t0, a.T);
     rd.load(dy, a.dys[1], t0, a.T);
-    const float* p = a.ckpt + (((int64_t)at.c * ntile + k) * a.B + at.b) * a.H + at.jr;
-#pragma unroll
-    for (int v = 0; v < V; ++v) hn[v] = p[v];
+    if (fore && onq) hn = a.ckpt[(((int64_t)at.c * ntile + k) * a.B + at.b) * a.H + jq];   // the state before the tile
   };
   load(k1 - 1);
   for (int k = k1 - 1; k >= k0; --k) {
-    const int t0 = k * kTile + at.grp * kSteps, buf = k & 1;
+    const int t0 = k * kTile + at.grp * kSteps;
     const uint32_t bits = real_bits<kSteps>(real);
-    float f[kSteps][V], keep[kSteps][V], xv[kSteps][V], d[kSteps][V], A[V], Bv[V], Gv[V];
+    float f[kSteps][V], keep[kSteps][V], xv[kSteps][V], d[kSteps][V];
     values<T, V, kSteps>(rx, rg, bits, f, keep, xv);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      A[v] = 1.f;
-      Bv[v] = Gv[v] = 0.f;
-    }
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       Vec<T, V>::get(rd.r[i], d[i]);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        d[i][v] = (bits >> i) & 1 ? d[i][v] : 0.f;
-        A[v] *= f[i][v];
-        Bv[v] = fmaf(f[i][v], Bv[v], keep[i][v] * xv[i][v]);
-      }
+      for (int v = 0; v < V; ++v) d[i][v] = (bits >> i) & 1 ? d[i][v] : 0.f;
     }
-#pragma unroll
-    for (int i = kSteps - 1; i >= 0; --i)
-#pragma unroll
-      for (int v = 0; v < V; ++v) Gv[v] = f[i][v] * (d[i][v] + Gv[v]);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      sA[buf][at.grp][at.lane * V + v] = A[v];
-      sB[buf][at.grp][at.lane * V + v] = Bv[v];
-      sG[buf][at.grp][at.lane * V + v] = Gv[v];
-      h[v] = hn[v];
-    }
+    float h = hn;
     if (k > k0) load(k - 1);
-    __syncthreads();
-    float s[V], e[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float tA[kGroups];
+      float A = 1.f, Bv = 0.f, Gv = 0.f;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        A *= f[i][v];
+        Bv = fmaf(f[i][v], Bv, keep[i][v] * xv[i][v]);
+      }
+#pragma unroll
+      for (int i = kSteps - 1; i >= 0; --i) Gv = f[i][v] * (d[i][v] + Gv);
+      sA[at.grp][at.lane * V + v] = A;
+      sB[at.grp][at.lane * V + v] = Bv;
+      sG[at.grp][at.lane * V + v] = Gv;
+    }
+    __syncthreads();
+    if (fore) {
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) {
-        tA[i] = sA[buf][i][at.lane * V + v];
-        if (i == at.grp) s[v] = h[v];
-        h[v] = fmaf(tA[i], h[v], sB[buf][i][at.lane * V + v]);
+        sS[i][q] = h;
+        h = fmaf(sA[i][q], h, sB[i][q]);
       }
+    } else if (aft) {
 #pragma unroll
       for (int i = kGroups - 1; i >= 0; --i) {
-        if (i == at.grp) e[v] = G[v];
-        G[v] = fmaf(tA[i], G[v], sG[buf][i][at.lane * V + v]);
+        sE[i][q] = G;
+        G = fmaf(sA[i][q], G, sG[i][q]);
       }
     }
-    // dgate without δ: (h_{t−1} − x_t) f_t (1 − f_t), formed on the way forward
-    float q[kSteps][V];
+    __syncthreads();
+    // dgate without δ, (h_{t−1} − x_t) f_t (1 − f_t), is formed on the way forward, in x's place
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i)
+    for (int v = 0; v < V; ++v) {
+      float s = sS[at.grp][at.lane * V + v];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        q[i][v] = (s[v] - xv[i][v]) * (f[i][v] * keep[i][v]);
-        s[v] = fmaf(f[i][v], s[v], keep[i][v] * xv[i][v]);
+      for (int i = 0; i < kSteps; ++i) {
+        const float n = fmaf(f[i][v], s, keep[i][v] * xv[i][v]);
+        xv[i][v] = (s - xv[i][v]) * (f[i][v] * keep[i][v]);
+        s = n;
       }
+    }
+    float e[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) e[v] = sE[at.grp][at.lane * V + v];
 #pragma unroll
     for (int i = kSteps - 1; i >= 0; --i) {
       float ox[V], og[V];
@@ -324,7 +318,7 @@ template <typename T, int V> __global__ __launch_bounds__(256) void bwd_kernel(c
       for (int v = 0; v < V; ++v) {
         const float dl = d[i][v] + e[v];
         ox[v] = keep[i][v] * dl;
-        og[v] = q[i][v] * dl;
+        og[v] = xv[i][v] * dl;
         e[v] = f[i][v] * dl;
       }
       if (at.on && t0 + i < a.T) {
@@ -333,9 +327,7 @@ template <typename T, int V> __global__ __launch_bounds__(256) void bwd_kernel(c
       }
     }
   }
-  if (at.on && at.grp == 0 && k0 == 0 && a.dh0)
-#pragma unroll
-    for (int v = 0; v < V; ++v) a.dh0[chan + v] = G[v];
+  if (aft && onq && k0 == 0 && a.dh0) a.dh0[seq * a.H + jq] = G;
 }
 
 // the map of every segment: forward h → A h + B (from x), backward G → A G + B (from dy)

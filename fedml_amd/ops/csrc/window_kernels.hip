@@ -820,7 +820,7 @@ __device__ __forceinline__ int slot_age(int s, int pos, int sinks, int W, int cu
 }
 
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW) void step_kernel(const StepArgs a) {
+__global__ __launch_bounds__(64 * NW, D * sizeof(T) > 256 ? 1 : 2) void step_kernel(const StepArgs a) {
   using R = Row<T, D>;
   __shared__ __attribute__((aligned(16))) T tiles[NW][2][32 * R::P];
   __shared__ float ml[NW][2][32];
@@ -860,10 +860,23 @@ __global__ __launch_bounds__(64 * NW) void step_kernel(const StepArgs a) {
   const int s0 = split * a.per, s1 = s0 + a.per < n ? s0 + a.per : n;
   constexpr int NI = 32 * R::U / 64;
   uint4 rk[NI], rv[NI];
+  const bool full = pos >= n - 1;                 // every slot holds a token
+  // a block of 32 slots whose rows all come from the cache
+  auto plain = [&](int base) { return full && base + 32 <= s1 && (cur < base || cur >= base + 32); };
   auto load = [&](int base) {
+    const int row = lane / R::U, c = (lane % R::U) * R::E;
+    if (plain(base)) {
+      const T *pk = kc + (int64_t)(base + row) * ld + c, *pv = vc + (int64_t)(base + row) * ld + c;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        rk[i] = *reinterpret_cast<const uint4*>(pk + (int64_t)(i * (64 / R::U)) * ld);
+        rv[i] = *reinterpret_cast<const uint4*>(pv + (int64_t)(i * (64 / R::U)) * ld);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int u = lane + 64 * i, s = base + u / R::U, c = (u % R::U) * R::E;
+      const int s = base + row + i * (64 / R::U);
       rk[i] = rv[i] = make_uint4(0, 0, 0, 0);
       if (s >= s1 || slot_age(s, pos, a.sinks, a.W, cur) < 0) continue;
       if (s == cur) {
@@ -880,6 +893,7 @@ __global__ __launch_bounds__(64 * NW) void step_kernel(const StepArgs a) {
     }
   };
   const float c2 = a.scale * kLog2e;
+  const float far = a.bias ? tab[(lane & 31) * a.NB + a.NB - 1] : 0.f;
   float m = -INFINITY, l = 0.f;
   f32x16 acc[R::DB];
 #pragma unroll
@@ -900,26 +914,35 @@ __global__ __launch_bounds__(64 * NW) void step_kernel(const StepArgs a) {
       if (base + 32 * NW < s1) load(base + 32 * NW);
       f32x16 s = R::rows(Ks, qf, ln);
       settle(s);
+      // whole blocks of the ring whose tokens are all max_distance old or older have one bias
+      const int last = base + 31, age = last < cur ? cur - last : a.W + cur - last;
+      if (plain(base) && (!a.bias || (base >= a.sinks && age >= a.maxd))) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int slot = base + kappa(r) + 4 * hh;
-        const int age = slot < s1 ? slot_age(slot, pos, a.sinks, a.W, cur) : -1;
-        float x = s[r] * c2;
-        if (a.bias && age >= 0) x += tab[(lane & 31) * a.NB + of[age < a.maxd ? age : a.maxd]];
-        s[r] = age >= 0 ? x : -INFINITY;
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, far);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int slot = base + kappa(r) + 4 * hh;
+          const int age = slot < s1 ? slot_age(slot, pos, a.sinks, a.W, cur) : -1;
+          float x = s[r] * c2;
+          if (a.bias && age >= 0) x += tab[(lane & 31) * a.NB + of[age < a.maxd ? age : a.maxd]];
+          s[r] = age >= 0 ? x : -INFINITY;
+        }
       }
       float mt = s[0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
       mt = half_max(mt);
-      const float mn = fmaxf(m, mt), mu = mn == -INFINITY ? 0.f : mn;
-      const float al = __builtin_amdgcn_exp2f(m - mu);
-      l *= al;
+      if (__any(mt > m + kGrow)) {
+        const float mn = fmaxf(m, mt), x = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= x;
 #pragma unroll
-      for (int db = 0; db < R::DB; ++db)
+        for (int db = 0; db < R::DB; ++db)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[db][r] *= al;
-      m = mn;
+          for (int r = 0; r < 16; ++r) acc[db][r] *= x;
+        m = mn;
+      }
+      const float mu = m == -INFINITY ? 0.f : m;
       float p[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -952,7 +975,8 @@ __global__ __launch_bounds__(64 * NW) void step_kernel(const StepArgs a) {
 #pragma unroll
   for (int db = 0; db < R::DB; ++db)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) mine[(lane & 31) * D + 32 * db + kappa(r) + 4 * hh] = acc[db][r] * al;
+    for (int r = 0; r < 16; ++r)
+      if (real) mine[(lane & 31) * D + 32 * db + kappa(r) + 4 * hh] = acc[db][r] * al;
   __syncthreads();
   // a column (head) of D sums at a time
   const int heads = G - grp * 32 < 32 ? G - grp * 32 : 32;

@@ -18,6 +18,10 @@ from ._launch import launch, ptr, ptr_read
 from .fl_ops import use_native
 
 _TILE = 32                # steps between two kept states
+# A call of fewer than _FULL workgroups cuts the time into segments, up to _WANT workgroups: x and gate are then read
+# twice. Forward + backward in us, whole / cut, at 64 workgroups (16384 steps): 1330 / 346; at 256: 361 / 353; at 384
+# (4096 steps): 495 / 541; more than 512 workgroups gain nothing.
+_FULL, _WANT = 256, 1024
 _I32 = 2 ** 31 - 1
 
 
@@ -54,7 +58,7 @@ def _run(a, x, gate, mask, streams, bwd):
         odd |= s0 | s1 | s2 | t.data_ptr() // es
     vec = 2 - (odd & 1)
     wgs, ntile = C * B * -(-H // (32 * vec)), -(-T // _TILE)
-    nseg = 1 if wgs >= 512 else min(ntile, -(-1024 // wgs), 64)
+    nseg = 1 if wgs >= _FULL else min(ntile, -(-_WANT // wgs), 64)
     a.tps = -(-ntile // (2 * nseg)) * 2        # pairs of tiles
     a.nseg = nseg = -(-ntile // a.tps)
     if wgs * nseg > _I32:

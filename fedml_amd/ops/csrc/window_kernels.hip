@@ -366,16 +366,31 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void fwd_kernel(const Arg
           for (int r = 0; r < 16; ++r) s[b][r] = fmaf(s[b][r], c2, far);
       }
     }
-    if (bits != ~0ull >> (64 - BK) || !block_whole(a, qw, k0, BK)) {
+    if (!block_whole(a, qw, k0, BK)) {
+      const int d = qi - k0 - 4 * hh;              // of the lane's first key; the window is 0 <= distance < W
+      if (k0 < a.sinks) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = 32 * b + kappa(r);
+            const bool see = d >= key && (d - key < a.W || k0 + 4 * hh + key < a.sinks);
+            s[b][r] = see ? s[b][r] : -INFINITY;
+          }
+      } else {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[b][r] = (uint32_t)(d - 32 * b - kappa(r)) < (uint32_t)a.W ? s[b][r] : -INFINITY;
+      }
+    }
+    if (bits != ~0ull >> (64 - BK)) {
       const uint64_t mine = bits >> (4 * hh);
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = k0 + 32 * b + kappa(r) + 4 * hh;
-          const bool see = key <= qi && (qi - key < a.W || key < a.sinks) && ((mine >> (32 * b + kappa(r))) & 1);
-          s[b][r] = see ? s[b][r] : -INFINITY;
-        }
+        for (int r = 0; r < 16; ++r) s[b][r] = (mine >> (32 * b + kappa(r))) & 1 ? s[b][r] : -INFINITY;
     }
     float mt = -INFINITY;
 #pragma unroll
@@ -512,7 +527,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
       sv.load(vp, a.ldv, tiles.at(it + 1) * BK, a.S - 1, tid);
     }
     if (!block_seen(a, qw, k0, BK)) continue;
-    const bool whole = bits == ~0ull >> (64 - BK) && block_whole(a, qw, k0, BK);
+    const bool whole = block_whole(a, qw, k0, BK);
 #pragma unroll
     for (int sub = 0; sub < BK / 32; ++sub) {
       const int kb = k0 + 32 * sub;
@@ -539,13 +554,22 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
 #pragma unroll
       for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(s[r]) * (dp[r] - Dq);
       if (!whole) {
+        const int d = qi - kb - 4 * hh;
+        if (kb < a.sinks) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const bool see = d >= kappa(r) && (d - kappa(r) < a.W || kb + 4 * hh + kappa(r) < a.sinks);
+            ds[r] = see ? ds[r] : 0.f;
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) ds[r] = (uint32_t)(d - kappa(r)) < (uint32_t)a.W ? ds[r] : 0.f;
+        }
+      }
+      if (bits != ~0ull >> (64 - BK)) {
         const uint32_t mine = (uint32_t)(bits >> (32 * sub)) >> (4 * hh);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = kb + kappa(r) + 4 * hh;
-          const bool see = key <= qi && (qi - key < a.W || key < a.sinks) && ((mine >> kappa(r)) & 1);
-          ds[r] = see ? ds[r] : 0.f;
-        }
+        for (int r = 0; r < 16; ++r) ds[r] = (mine >> kappa(r)) & 1 ? ds[r] : 0.f;
       }
       R::cols(acc, Ks + 32 * sub * R::P, ds, ln);
       if (BIAS) {
@@ -639,7 +663,6 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
     qe = (int64_t)k0 + 32 * NW - 1 + a.W < a.S ? k0 + 32 * NW - 1 + a.W : a.S;
   }
   const int nt = (qe - qs + BQ - 1) / BQ;
-  const bool allreal = !__any(!real);
   const int count = __syncthreads_or(real) ? nt * G : 0;
   const float c2 = a.scale * kLog2e;
   f32x16 ak[R::DB], av[R::DB];
@@ -673,7 +696,7 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
     if (a.bias && it % nt == 0) fill_lut(lut, a, n / (a.N / a.C), kv * G + it / nt, tid, 64 * NW);
     __syncthreads();
     if (it + 1 < count) load(it + 1);
-    const bool whole = allreal && (sink ? q0 - kw - 31 >= a.W : q0 >= kw + 31 && q0 + BQ - 1 - kw < a.W);
+    const bool whole = sink ? q0 - kw - 31 >= a.W : q0 >= kw + 31 && q0 + BQ - 1 - kw < a.W;
 #pragma unroll
     for (int sub = 0; sub < BQ / 32; ++sub) {
       const int qb = q0 + 32 * sub;
@@ -709,8 +732,8 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
       if (!whole) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int d = qb + kappa(r) + 4 * hh - kj;
-          const bool see = real && d >= 0 && (sink ? d >= a.W : d < a.W);
+          const int d = qb + 4 * hh - kj + kappa(r);
+          const bool see = sink ? d >= a.W : (uint32_t)d < (uint32_t)a.W;
           p[r] = see ? p[r] : 0.f;
           ds[r] = see ? ds[r] : 0.f;
         }
@@ -722,6 +745,10 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
 #pragma unroll
   for (int db = 0; db < R::DB; ++db) settle(ak[db], av[db]);
   if (kj >= a.S || (sink && kj >= a.sinks)) return;
+  if (!real) {                                   // a column of no token: whatever its sums are, it has no gradient
+#pragma unroll
+    for (int db = 0; db < R::DB; ++db) ak[db] = av[db] = zero16();
+  }
   if (a.nchunk && kj < a.sinks) {
     float* pk = a.part + ((((int64_t)n * a.KV + kv) * (a.nchunk + 1) + (sink ? chunk + 1 : 0)) * 2 * a.sinks + kj) * D +
                 4 * hh;

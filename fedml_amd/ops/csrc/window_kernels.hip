@@ -27,6 +27,7 @@ typedef short v4i16 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMfma = 0x8, kDsRead = 0x100;      // classes of instructions for the scheduler
 constexpr float kGrow = 8.f;      // see fwd_kernel
 constexpr int kMaxBuckets = 128;
 constexpr int kLutOff = 94;      // a processed block of 32 queries and <= 64 keys holds distances >= −94 (the negative
@@ -192,45 +193,86 @@ template <typename T, int D> struct Row {
 #pragma unroll
     for (int c = 0; c < NC; ++c) f[c] = real ? unit(row, 2 * c + hh) : make_uint4(0, 0, 0, 0);
   }
-  // 32 rows of an LDS tile × this lane's column: Σ over the head dim
+  // s0 and s1 += 32 rows each of two LDS tiles × this lane's columns: Σ over the head dim. DEEP: one tile's reads are all
+  // in flight before its first product, the other's are made between those (left to itself the compiler keeps two in
+  // flight, and every pair of products waits for LDS); it takes 2·NC·4 registers.
+  template <bool DEEP> static __device__ __forceinline__ void rows2(f32x16& s0, f32x16& s1, const T* t0, const T* t1, const uint4* f0,
+                                               const uint4* f1, const Lane& ln) {
+    uint4 x[NC], y[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) x[c] = *reinterpret_cast<const uint4*>(t0 + ln.row[c]);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) y[c] = *reinterpret_cast<const uint4*>(t1 + ln.row[c]);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) s0 = Elem<T>::mma(x[c], f0[c], s0);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) s1 = Elem<T>::mma(y[c], f1[c], s1);
+    if constexpr (sizeof(T) == 2 && DEEP) {
+      __builtin_amdgcn_sched_group_barrier(kDsRead, NC, 0);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(kMfma, NC, 0);
+    }
+    settle(s0, s1);
+  }
   static __device__ __forceinline__ f32x16 rows(const T* tile, const uint4* f, const Lane& ln) {
     f32x16 acc = zero16();
+    uint4 x[NC];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) acc = Elem<T>::mma(*reinterpret_cast<const uint4*>(tile + ln.row[c]), f[c], acc);
+    for (int c = 0; c < NC; ++c) x[c] = *reinterpret_cast<const uint4*>(tile + ln.row[c]);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc = Elem<T>::mma(x[c], f[c], acc);
+    if constexpr (sizeof(T) == 2) {
+      __builtin_amdgcn_sched_group_barrier(kDsRead, NC, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, NC, 0);
+    }
+    settle(acc);
     return acc;
   }
-  // acc[db][column][row] += Σ over 32 rows of the LDS tile of tile[row][32 db + ·] · p[row]
-  static __device__ __forceinline__ void cols(f32x16* acc, const T* tile, const float* p, const Lane& ln) {
-    if constexpr (sizeof(T) == 2) {
-      bf16x8 b[2];
+  // acc[db][column][row] += Σ over 32 rows of the LDS tile of tile[row][32 db + ·] · p[row]. bf16: read() takes the
+  // tile's fragments, ahead of the work that gives p
+  struct Cols {
+    const T* tile;
+    bf16x8 f[sizeof(T) == 2 ? 2 * (D / 32) : 1];
+    __device__ __forceinline__ void read(const T* t, const Lane& ln) {
+      tile = t;
+      if constexpr (sizeof(T) == 2) {
+        const uint16_t* base = reinterpret_cast<const uint16_t*>(t);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) b[t][j] = (__bf16)p[8 * t + j];
-      const uint16_t* base = reinterpret_cast<const uint16_t*>(tile);
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {      // swz(row + 16) = swz(row)
-          const v4i16 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(base + 16 * t * P + ln.col[2 * db]));
-          const v4i16 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(base + 16 * t * P + ln.col[2 * db + 1]));
+        for (int k = 0; k < 2 * DB; ++k) {      // column block k / 2, rows 16 (k & 1) …; swz(row + 16) = swz(row)
           union {
             v4i16 h[2];
             bf16x8 v;
           } a;
-          a.h[0] = x;
-          a.h[1] = y;
-          acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b[t], acc[db], 0, 0, 0);
+          a.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(base + 16 * (k & 1) * P + ln.col[k & ~1]));
+          a.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(base + 16 * (k & 1) * P + ln.col[k | 1]));
+          f[k] = a.v;
         }
-    } else {
-      const float* base = reinterpret_cast<const float*>(tile) + ln.col[0];
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-          acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(base[kappa(r) * P + 32 * db], p[r], acc[db], 0, 0, 0);
+      }
     }
-  }
+    __device__ __forceinline__ void mul(f32x16* acc, const float* p, const Lane& ln) const {
+      if constexpr (sizeof(T) == 2) {
+        bf16x8 b[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) b[t][j] = (__bf16)p[8 * t + j];
+#pragma unroll
+        for (int k = 0; k < 2 * DB; ++k)
+          acc[k / 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[k], b[k & 1], acc[k / 2], 0, 0, 0);
+      } else {
+        const float* base = reinterpret_cast<const float*>(tile) + ln.col[0];
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+            acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(base[kappa(r) * P + 32 * db], p[r], acc[db], 0, 0, 0);
+      }
+    }
+  };
 };
 
 // ROWS rows of a [·][D] source between registers and an LDS tile, NT threads. Loads are unconditional, of rows up to
@@ -346,10 +388,12 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void fwd_kernel(const Arg
     constexpr int NB = BK / 32;
     if (!block_seen(a, qw, k0, BK)) continue;
     f32x16 s[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) s[b] = R::rows(Ks + 32 * b * R::P, qf, ln);
-    if constexpr (NB == 2) settle(s[0], s[1]);
-    else settle(s[0]);
+    if constexpr (NB == 2) {
+      s[0] = s[1] = zero16();
+      R::template rows2<true>(s[0], s[1], Ks, Ks + 32 * R::P, qf, qf, ln);
+    } else {
+      s[0] = R::rows(Ks, qf, ln);
+    }
     if (BIAS) {
       if (qw - k0 - (BK - 1) < a.maxd) {
 #pragma unroll
@@ -412,19 +456,21 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void fwd_kernel(const Arg
     const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+      typename R::Cols vt;
+      vt.read(Vs + 32 * b * R::P, ln);
       float p[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         p[r] = __builtin_amdgcn_exp2f(BIAS ? s[b][r] - mu : fmaf(s[b][r], c2, -mu));
         l += p[r];
       }
-      R::cols(acc, Vs + 32 * b * R::P, p, ln);
+      vt.mul(acc, p, ln);
       if (EXACT) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) p[r] = Elem<T>::left(p[r]);
-          R::cols(acc, Vs + 32 * b * R::P, p, ln);
+          vt.mul(acc, p, ln);
         }
       }
     }
@@ -532,9 +578,8 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
     for (int sub = 0; sub < BK / 32; ++sub) {
       const int kb = k0 + 32 * sub;
       if (!block_seen(a, qw, kb, 32)) continue;
-      f32x16 s = R::rows(Ks + 32 * sub * R::P, qf, ln);
-      f32x16 dp = R::rows(Vs + 32 * sub * R::P, df, ln);
-      settle(s, dp);
+      f32x16 s = zero16(), dp = zero16();
+      R::template rows2<D * sizeof(T) <= 128>(s, dp, Ks + 32 * sub * R::P, Vs + 32 * sub * R::P, qf, df, ln);
       const bool near = BIAS && qw - kb - 31 < a.maxd;
       if (BIAS) {
         if (near) {
@@ -571,7 +616,9 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
 #pragma unroll
         for (int r = 0; r < 16; ++r) ds[r] = (mine >> kappa(r)) & 1 ? ds[r] : 0.f;
       }
-      R::cols(acc, Ks + 32 * sub * R::P, ds, ln);
+      typename R::Cols kt;      // read ahead of ds it would cost a wave of occupancy (D 64) or spill (D 128)
+      kt.read(Ks + 32 * sub * R::P, ln);
+      kt.mul(acc, ds, ln);
       if (BIAS) {
         if (near) {
           float* at = sk_w + (lane & 31) * 65 + 31 - 4 * hh;       // row i, column i − key + 31
@@ -702,9 +749,10 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
       const int qb = q0 + 32 * sub;
       if (kw >= a.S || qb >= qe || qb + 31 < kw) continue;
       if (sink ? (kw >= a.sinks || qb + 31 - kw < a.W) : qb - kw - 31 >= a.W) continue;
-      f32x16 s = R::rows(Qs + 32 * sub * R::P, kf, ln);
-      f32x16 dp = R::rows(Os + 32 * sub * R::P, vf, ln);
-      settle(s, dp);
+      f32x16 s = zero16(), dp = zero16();
+      R::template rows2<true>(s, dp, Qs + 32 * sub * R::P, Os + 32 * sub * R::P, kf, vf, ln);
+      typename R::Cols ot, qt;
+      ot.read(Os + 32 * sub * R::P, ln);
       if (a.bias) {
         if (qb - kw - 31 < a.maxd) {
           const float* at = lut + kLutOff + qb - kj + 4 * hh;
@@ -738,8 +786,9 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
           ds[r] = see ? ds[r] : 0.f;
         }
       }
-      R::cols(av, Os + 32 * sub * R::P, p, ln);
-      R::cols(ak, Qs + 32 * sub * R::P, ds, ln);
+      qt.read(Qs + 32 * sub * R::P, ln);
+      ot.mul(av, p, ln);
+      qt.mul(ak, ds, ln);
     }
   }
 #pragma unroll
@@ -940,7 +989,6 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 256 ? 1 : 2) void step_ker
       __builtin_amdgcn_wave_barrier();
       if (base + 32 * NW < s1) load(base + 32 * NW);
       f32x16 s = R::rows(Ks, qf, ln);
-      settle(s);
       // whole blocks of the ring whose tokens are all max_distance old or older have one bias
       const int last = base + 31, age = last < cur ? cur - last : a.W + cur - last;
       if (plain(base) && (!a.bias || (base >= a.sinks && age >= a.maxd))) {
@@ -976,7 +1024,9 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 256 ? 1 : 2) void step_ker
         p[r] = __builtin_amdgcn_exp2f(s[r] - mu);
         l += p[r];
       }
-      R::cols(acc, Vs, p, ln);
+      typename R::Cols vt;
+      vt.read(Vs, ln);
+      vt.mul(acc, p, ln);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }

@@ -44,6 +44,7 @@ struct Args {
   int N, S, H, KV, C, W, sinks, NB, maxd;
   int nchunk, qchunk;            // sink pass of the backward: chunks of queries
   int exact;                     // forward: a gradient of the bias follows
+  int tile;                      // queries of a workgroup, forward and dq: 32 or 128
   float scale;
   int start[kMaxBuckets];        // first distance of every bucket
 };
@@ -700,14 +701,15 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
   uint4 kf[R::NC], vf[R::NC];
   R::frags(kf, (const T*)a.k + (tok0 + kj) * a.ldk + kv * D, real, hh);
   R::frags(vf, (const T*)a.v + (tok0 + kj) * a.ldv + kv * D, real, hh);
-  // queries [qs, qe): through the window, or a chunk of those beyond it
+  // queries [qs, qe): through the window (and to the end where the sinks have no pass of their own), or a chunk beyond
+  const int own = a.nchunk ? 0 : a.sinks;
   int qs, qe;
   if (sink) {
     qs = a.W + chunk * a.qchunk;
     qe = qs + a.qchunk < a.S ? qs + a.qchunk : a.S;
   } else {
     qs = k0;
-    qe = (int64_t)k0 + 32 * NW - 1 + a.W < a.S ? k0 + 32 * NW - 1 + a.W : a.S;
+    qe = k0 >= own && (int64_t)k0 + 32 * NW - 1 + a.W < a.S ? k0 + 32 * NW - 1 + a.W : a.S;
   }
   const int nt = (qe - qs + BQ - 1) / BQ;
   const int count = __syncthreads_or(real) ? nt * G : 0;
@@ -743,12 +745,12 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
     if (a.bias && it % nt == 0) fill_lut(lut, a, n / (a.N / a.C), kv * G + it / nt, tid, 64 * NW);
     __syncthreads();
     if (it + 1 < count) load(it + 1);
-    const bool whole = sink ? q0 - kw - 31 >= a.W : q0 >= kw + 31 && q0 + BQ - 1 - kw < a.W;
+    const bool whole = sink ? q0 - kw - 31 >= a.W : q0 >= kw + 31 && (q0 + BQ - 1 - kw < a.W || kw + 31 < own);
 #pragma unroll
     for (int sub = 0; sub < BQ / 32; ++sub) {
       const int qb = q0 + 32 * sub;
       if (kw >= a.S || qb >= qe || qb + 31 < kw) continue;
-      if (sink ? (kw >= a.sinks || qb + 31 - kw < a.W) : qb - kw - 31 >= a.W) continue;
+      if (sink ? (kw >= a.sinks || qb + 31 - kw < a.W) : (qb - kw - 31 >= a.W && kw >= own)) continue;
       f32x16 s = zero16(), dp = zero16();
       R::template rows2<true>(s, dp, Qs + 32 * sub * R::P, Os + 32 * sub * R::P, kf, vf, ln);
       typename R::Cols ot, qt;
@@ -781,7 +783,7 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int d = qb + 4 * hh - kj + kappa(r);
-          const bool see = sink ? d >= a.W : (uint32_t)d < (uint32_t)a.W;
+          const bool see = sink ? d >= a.W : (uint32_t)d < (uint32_t)a.W || (kj < own && d >= 0);
           p[r] = see ? p[r] : 0.f;
           ds[r] = see ? ds[r] : 0.f;
         }
@@ -1140,7 +1142,7 @@ template <typename T, int D, int NW, int BK> int launch_fwd_tile(const Args& a, 
 }
 
 template <typename T, int D> int launch_fwd(const Args& a, hipStream_t st) {
-  if (a.S > 64) return launch_fwd_tile<T, D, 4, sizeof(T) == 2 ? 64 : 32>(a, st);
+  if (a.tile == 128) return launch_fwd_tile<T, D, 4, sizeof(T) == 2 ? 64 : 32>(a, st);
   return launch_fwd_tile<T, D, 1, 32>(a, st);
 }
 
@@ -1158,21 +1160,21 @@ template <typename T, int D, int NW, int BK> int launch_dq(const Args& a, hipStr
 template <typename T, int D> int launch_bwd(const Args& a, hipStream_t st) {
   const size_t lds = a.bias ? (a.maxd + 2 * kLutOff) * sizeof(float) : 0;
   int rc;
-  if (a.S > 64) rc = launch_dq<T, D, 4, sizeof(T) == 2 ? 64 : 32>(a, st);
+  if (a.tile == 128) rc = launch_dq<T, D, 4, sizeof(T) == 2 ? 64 : 32>(a, st);
   else rc = launch_dq<T, D, 1, 32>(a, st);
   if (rc) return rc;
   const int64_t nsink = (int64_t)a.nchunk * a.N * a.KV;
   // 64 keys suffice for a short sequence; at fp32 and 128 dims two waves would have to spill
   constexpr int kFew = D * sizeof(T) > 256 ? 4 : 2;
-  if (a.S > 64) {
+  if (a.tile == 128) {
     const int64_t n = nsink + (int64_t)a.N * a.KV * ((a.S + 127) / 128);
     hipLaunchKernelGGL((dkv_kernel<T, D, 4, sizeof(T) == 2 ? 64 : 32>), dim3((unsigned)n), dim3(256), lds, st, a);
   } else {
-    const int64_t n = nsink + (int64_t)a.N * a.KV;
+    const int64_t n = nsink + (int64_t)a.N * a.KV * ((a.S + 32 * kFew - 1) / (32 * kFew));
     hipLaunchKernelGGL((dkv_kernel<T, D, kFew, 32>), dim3((unsigned)n), dim3(64 * kFew), lds, st, a);
   }
   if ((rc = (int)hipGetLastError())) return rc;
-  const int nqt = a.S > 64 ? (a.S + 127) / 128 : (a.S + 31) / 32;
+  const int nqt = (a.S + a.tile - 1) / a.tile;
   const int64_t blocks = (a.dbias ? (int64_t)a.C * a.H : 0) +
                          (a.nchunk ? ((int64_t)a.N * a.KV * 2 * a.sinks * (D / 4) + 255) / 256 : 0);
   if (blocks) hipLaunchKernelGGL(finish_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, a, D, nqt);

@@ -34,7 +34,7 @@ class _Args(_c.Structure):
     _fields_ = [(n, _c.c_void_p) for n in ("q", "k", "v", "dout", "o", "dq", "dk", "dv", "o32", "lse", "dsum", "part",
                                            "bpart", "dbias", "mask", "bias")] + \
                [(n, _c.c_int64) for n in ("ldq", "ldk", "ldv", "lddo")] + \
-               [(n, _c.c_int) for n in ("N", "S", "H", "KV", "C", "W", "sinks", "NB", "maxd", "nchunk", "qchunk", "exact")] + \
+               [(n, _c.c_int) for n in ("N", "S", "H", "KV", "C", "W", "sinks", "NB", "maxd", "nchunk", "qchunk", "exact", "tile")] + \
                [("scale", _c.c_float), ("start", _c.c_int * MAX_BUCKETS)]
 
 
@@ -176,13 +176,21 @@ def _window_ref(q, k, v, S, H, KV, W, sinks, mask, bias, max_distance, scale):
 
 # --------------------------------------------------------------------------------------------------------- training
 @functools.lru_cache(maxsize=256)
-def _plan(N, S, H, KV, W, sinks, scale, C, buckets, max_distance):
+def _plan(N, S, H, KV, W, sinks, scale, fp32, C, buckets, max_distance):
     """What the kernels' arguments hold for all calls of these sizes."""
     a = _Args(N=N, S=S, H=H, KV=KV, C=C, W=W, sinks=sinks, NB=buckets, scale=scale)
     if buckets:
         a.maxd = max_distance
         a.start[:buckets] = relative_bucket_starts(buckets, max_distance)
-    if sinks and S > W:                     # the sink pass: chunks of queries about as long as a window's walk
+    # Queries of a workgroup, forward and dq: one wave's 32 for short sequences, and at fp32, where products are 16 times
+    # as long, wherever no more than 1024 such waves are there (a wave then walks its own keys, not its workgroup's).
+    # us forward + backward, 128 / 32 queries: fp32 [80·80, 4 heads] 19 + 73 / 15 + 72, [16·256, 4] 23 + 81 / 17 + 72,
+    # [64·128, 12] 37 + 152 / 45 + 163; bf16 [16·256, 4] 10 + 31 / 8 + 30, [2·2048, 8] 19 + 59 / 23 + 71.
+    a.tile = 32 if S <= 64 or (fp32 and N * H * -(-S // 32) <= 1024) else 128
+    # The sinks' gradients from behind their window: up to 512 queries are walked by the sinks' own keys, more by a pass
+    # of its own in chunks about as long as a window's walk ([80·80, 4 heads] fp32, 48 such queries: dk/dv 54 us with
+    # the pass, 45 without).
+    if sinks and S - W > 512:
         a.qchunk = max(512, -(-(W + 128) // 128) * 128)
         a.nchunk = -(-(S - W) // a.qchunk)
     return a
@@ -241,8 +249,7 @@ class _WindowAttention(torch.autograd.Function):
             if a.nchunk:
                 part = torch.empty(N, KV, a.nchunk + 1, 2, a.sinks, D, dtype=f32, device=dev)
             if dbias is not None:
-                tile = 128 if S > 64 else 32                  # queries of a workgroup of the dq kernel
-                bpart = torch.empty(N, H, -(-S // tile), bias.shape[-1], dtype=f32, device=dev)
+                bpart = torch.empty(N, H, -(-S // a.tile), bias.shape[-1], dtype=f32, device=dev)
             a.dout, a.lddo, a.lse, a.o32 = ptr_read(do), do.stride(0), ptr_read(lse), ptr_read(o32)
             a.dq, a.dk, a.dv, a.dsum = ptr(dq), ptr(dk), ptr(dv), ptr(dsum)
             a.part, a.bpart, a.dbias = ptr(part), ptr(bpart), ptr(dbias)
@@ -280,8 +287,8 @@ def window_attention(q, k, v, S: int, H: int, window: int, sinks: int = 0, kv_he
         return _window_ref(q, k, v, S, H, KV, W, sinks, mask, table, max_distance, scale)
     if mask is not None:
         mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous().view(torch.uint8)
-    cfg = (D, N, S, H, KV, min(W, S), min(sinks, S), scale, *((0, 0, 0) if table is None else
-                                                              (table.shape[0], table.shape[2], int(max_distance))))
+    cfg = (D, N, S, H, KV, min(W, S), min(sinks, S), scale, q.dtype == torch.float32,
+           *((0, 0, 0) if table is None else (table.shape[0], table.shape[2], int(max_distance))))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
                                     (table is not None and table.requires_grad)):
         return _WindowAttention.apply(q, k, v, table, mask, cfg)
@@ -299,6 +306,8 @@ def _cache(k_cache, v_cache, B, KV, D, slots, dtype, device):
             raise ValueError(f"{n}: contiguous, 16-byte aligned memory expected (it is updated in place)")
         if t.requires_grad:
             raise ValueError(f"{n} takes no gradient")
+    if k_cache.numel() and k_cache.data_ptr() == v_cache.data_ptr():
+        raise ValueError("k_cache and v_cache are the same memory")
 
 
 def _pos(pos, B, device, name):

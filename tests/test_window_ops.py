@@ -189,6 +189,9 @@ def test_step_refusals(error, match, kw):
     a.update(kw)
     with pytest.raises(error, match=match):
         ops.window_attention_step(**a)
+    with pytest.raises(ValueError, match="same memory"):
+        c = _t(2, 5, 128)
+        ops.window_attention_step(_t(2, 128), _t(2, 128), _t(2, 128), c, c, torch.zeros(2, dtype=torch.int32), 2, 4, 1)
 
 
 @pytest.mark.parametrize("error,match,kw", [

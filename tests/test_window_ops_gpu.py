@@ -133,7 +133,10 @@ CASES = [  # N, S, H, KV, D, window, sinks, mask, C, NB, M
     (2, 127, 2, 2, 64, 32, 1, "right", 2, 16, 64), (1, 129, 6, 2, 64, 16, 4, None, 1, 32, 128),
     (2, 200, 2, 1, 128, 1, 3, "right", 0, 0, 0), (1, 300, 2, 1, 64, 300, 0, None, 1, 2, 1024),
     (1, 300, 2, 2, 64, 47, 64, None, 1, 128, 300), (4, 61, 2, 1, 64, 9, 40, "right", 4, 5, 9),
-    (1, 257, 8, 1, 128, 64, 0, None, 1, 8, 32), (2, 300, 2, 1, 64, 31, 31, "holes", 2, 3, 500)]
+    (1, 257, 8, 1, 128, 64, 0, None, 1, 8, 32), (2, 300, 2, 1, 64, 31, 31, "holes", 2, 3, 500),
+    # enough heads for workgroups of 128 queries at fp32 too
+    (40, 130, 8, 4, 64, 48, 3, "right", 2, 16, 64), (30, 140, 8, 2, 128, 33, 64, "holes", 0, 0, 0),
+    (26, 150, 9, 3, 128, 150, 0, None, 1, 32, 128)]
 
 
 def _call(ops_args, q, k, v, bias, do):
@@ -169,13 +172,16 @@ def test_forward_and_gradients(case, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
-def test_long_rows_against_short_windows(dtype):
-    """Thousands of tokens: the sinks' gradients come from many chunks of queries."""
-    N, S, H, KV, D, window, sinks = 1, 2900, 2, 1, 64, 40, 3
+@pytest.mark.parametrize("N,S,H,KV,D,window,sinks,kind,C", [
+    (1, 2900, 2, 1, 64, 40, 3, None, 1), (1, 1100, 2, 2, 128, 70, 64, "right", 0), (2, 1400, 14, 7, 64, 100, 33, "right", 2),
+    (1, 1200, 30, 10, 128, 129, 1, "holes", 0)])
+def test_long_rows_against_short_windows(N, S, H, KV, D, window, sinks, kind, C, dtype):
+    """Many more tokens than the window: the sinks' gradients come from chunks of queries."""
     q, k, v, do = _data(N, S, H, KV, D, dtype, 5)
-    bias = torch.randn(1, H, 16, generator=torch.Generator().manual_seed(3)).to(dev)
-    got = _call((S, H, window, sinks, KV, None, 100, None), q, k, v, bias, do)
-    want = _oracle(q, k, v, do, S, H, KV, window, sinks, None, bias, 100, D ** -0.5, dtype)
+    bias = torch.randn(C, H, 16, generator=torch.Generator().manual_seed(3)).to(dev) if C else None
+    mask = _mask(kind, N, S)
+    got = _call((S, H, window, sinks, KV, mask, 100, None), q, k, v, bias, do)
+    want = _oracle(q, k, v, do, S, H, KV, window, sinks, mask, bias, 100, D ** -0.5, dtype)
     for g, w, name in zip(got, want, ("o", "dq", "dk", "dv", "dbias")):
         _within(g, w, name)
 

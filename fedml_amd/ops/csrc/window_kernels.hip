@@ -16,6 +16,18 @@
 //   chunk is the same on both sides, so the sum is over all of them;
 //   column operands (products over 32 rows of an LDS tile): the 16 accumulators of a lane ARE the other operand,
 //   with the rows taken in the order κ(r) + 4·hh, so probabilities never leave the registers.
+//
+// Measured on MI355X (a large copy reaches 4.94 TB/s, an 8192³ product 1420 TFLOP/s bf16 and 154 fp32):
+//   forward, bf16:  32768 tokens, 32 heads over 8, D 128, W 1024: 770 us = 714 TFLOP/s; 16 · 1999 (a quarter padding),
+//                   12 heads, D 64, W 256: 98 us
+//   dq / dk, dv:    2 · 16384, 16 heads over 4, D 128, W 1024: 520 / 1040 us = 793 / 529 TFLOP/s of the products they
+//                   make (3 and 4 a block); 16 · 1999 as above: 102 / 167 us
+//   step, bf16:     64 caches of 4100 slots, 32 heads over 8, D 128: 225 us = 4.8 TB/s
+// A 32×32 block at D 128 takes the matrix unit 512 cycles forward, 768 in dq and 1024 in dk/dv, the vector unit about
+// 500 in each (16 exponentials a lane at a quarter rate, and what stands around them): the two share the time of a wave,
+// and only other waves of the SIMD fill it — two of them in the forward and dq, one in dk/dv, whose sums, keys and
+// values take 416 registers (keys and values in LDS with two waves a SIMD: 1091 us; two blocks interleaved: spills,
+// 1407 us). At D 64 short windows add the tiles at their edges, which are masked, and a tile's latency at either end.
 #include "common.h"
 #include <type_traits>
 
@@ -332,6 +344,9 @@ struct KeyTiles {
 // ----------------------------------------------------------------------------------------------------------------
 // Forward: a wave owns 32 queries (its columns), the workgroup 32·NW of one head, and walks the visible keys in tiles
 // of BK with a running maximum and sum. The next tile's rows are in flight in registers during a tile's products.
+// 64 keys at bf16: with 32, an iteration was shorter than a load's latency (dq, 16k tokens: 1105 us instead of 561);
+// 256 queries a workgroup are no faster at D 128 and a quarter slower at D 64. At fp32 32 keys keep the registers for
+// two waves a SIMD, and a block's products (4096 cycles at D 64) cover the latency.
 // Probabilities are rounded to the storage type for the product with v (half a step each, 2^-8 in bf16, and the sum is
 // of the unrounded ones). EXACT (bf16, before a gradient of the bias): what that rounding leaves over goes through a
 // second product, so that D = dO·o of the unrounded output is good to 2^-16 — dbias is fp32.
@@ -780,12 +795,22 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
         }
       }
       if (!whole) {
+        const int d = qb + 4 * hh - kj;
+        if (sink || kw < own) {
+          const int least = sink ? a.W : 0, most = !sink && kj >= own ? a.W : 0x7fffffff;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int d = qb + 4 * hh - kj + kappa(r);
-          const bool see = sink ? d >= a.W : (uint32_t)d < (uint32_t)a.W || (kj < own && d >= 0);
-          p[r] = see ? p[r] : 0.f;
-          ds[r] = see ? ds[r] : 0.f;
+          for (int r = 0; r < 16; ++r) {
+            const bool see = d + kappa(r) >= least && d + kappa(r) < most;
+            p[r] = see ? p[r] : 0.f;
+            ds[r] = see ? ds[r] : 0.f;
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const bool see = (uint32_t)(d + kappa(r)) < (uint32_t)a.W;
+            p[r] = see ? p[r] : 0.f;
+            ds[r] = see ? ds[r] : 0.f;
+          }
         }
       }
       qt.read(Qs + 32 * sub * R::P, ln);

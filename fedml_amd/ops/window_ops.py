@@ -275,8 +275,8 @@ def window_attention(q, k, v, S: int, H: int, window: int, sinks: int = 0, kv_he
     if S < 1 or q.shape[0] % S:
         raise ValueError(f"{q.shape[0]} rows are no whole sequences of {S} tokens")
     N = q.shape[0] // S
-    if N * S > _I32 or N * H * S > _I32:
-        raise ValueError(f"{N} sequences · {H} heads · {S} tokens: at most 2^31 − 1")
+    if N * H * S > _I32 or S > 2 ** 30:
+        raise ValueError(f"{N} sequences · {H} heads · {S} tokens: at most 2^31 − 1 in all, 2^30 a sequence")
     if mask is not None:
         if mask.shape != (N, S) or mask.dtype.is_floating_point or mask.dtype.is_complex or mask.device != q.device:
             raise ValueError(f"mask: bool or integer [{N}, {S}] on {q.device} expected, got {mask.dtype} "

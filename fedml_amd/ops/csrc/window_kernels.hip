@@ -56,7 +56,7 @@ struct Args {
   int N, S, H, KV, C, W, sinks, NB, maxd;
   int nchunk, qchunk;            // sink pass of the backward: chunks of queries
   int exact;                     // forward: a gradient of the bias follows
-  int tile;                      // queries of a workgroup, forward and dq: 32 or 128
+  int tile, ktile;               // a workgroup's queries, forward and dq: 32 or 128; its keys, dk and dv: 64 or 128
   float scale;
   int start[kMaxBuckets];        // first distance of every bucket
 };
@@ -1189,14 +1189,13 @@ template <typename T, int D> int launch_bwd(const Args& a, hipStream_t st) {
   else rc = launch_dq<T, D, 1, 32>(a, st);
   if (rc) return rc;
   const int64_t nsink = (int64_t)a.nchunk * a.N * a.KV;
-  // 64 keys suffice for a short sequence; at fp32 and 128 dims two waves would have to spill
-  constexpr int kFew = D * sizeof(T) > 256 ? 4 : 2;
-  if (a.tile == 128) {
-    const int64_t n = nsink + (int64_t)a.N * a.KV * ((a.S + 127) / 128);
+  const int64_t n = nsink + (int64_t)a.N * a.KV * ((a.S + a.ktile - 1) / a.ktile);
+  if (a.ktile == 128) {
     hipLaunchKernelGGL((dkv_kernel<T, D, 4, sizeof(T) == 2 ? 64 : 32>), dim3((unsigned)n), dim3(256), lds, st, a);
+  } else if constexpr (D * sizeof(T) <= 256) {
+    hipLaunchKernelGGL((dkv_kernel<T, D, 2, 32>), dim3((unsigned)n), dim3(128), lds, st, a);
   } else {
-    const int64_t n = nsink + (int64_t)a.N * a.KV * ((a.S + 32 * kFew - 1) / (32 * kFew));
-    hipLaunchKernelGGL((dkv_kernel<T, D, kFew, 32>), dim3((unsigned)n), dim3(64 * kFew), lds, st, a);
+    return (int)hipErrorInvalidValue;
   }
   if ((rc = (int)hipGetLastError())) return rc;
   const int nqt = (a.S + a.tile - 1) / a.tile;

@@ -34,7 +34,8 @@ class _Args(_c.Structure):
     _fields_ = [(n, _c.c_void_p) for n in ("q", "k", "v", "dout", "o", "dq", "dk", "dv", "o32", "lse", "dsum", "part",
                                            "bpart", "dbias", "mask", "bias")] + \
                [(n, _c.c_int64) for n in ("ldq", "ldk", "ldv", "lddo")] + \
-               [(n, _c.c_int) for n in ("N", "S", "H", "KV", "C", "W", "sinks", "NB", "maxd", "nchunk", "qchunk", "exact", "tile")] + \
+               [(n, _c.c_int) for n in ("N", "S", "H", "KV", "C", "W", "sinks", "NB", "maxd", "nchunk", "qchunk", "exact",
+                                        "tile", "ktile")] + \
                [("scale", _c.c_float), ("start", _c.c_int * MAX_BUCKETS)]
 
 
@@ -176,7 +177,7 @@ def _window_ref(q, k, v, S, H, KV, W, sinks, mask, bias, max_distance, scale):
 
 # --------------------------------------------------------------------------------------------------------- training
 @functools.lru_cache(maxsize=256)
-def _plan(N, S, H, KV, W, sinks, scale, fp32, C, buckets, max_distance):
+def _plan(D, N, S, H, KV, W, sinks, scale, fp32, C, buckets, max_distance):
     """What the kernels' arguments hold for all calls of these sizes."""
     a = _Args(N=N, S=S, H=H, KV=KV, C=C, W=W, sinks=sinks, NB=buckets, scale=scale)
     if buckets:
@@ -187,6 +188,10 @@ def _plan(N, S, H, KV, W, sinks, scale, fp32, C, buckets, max_distance):
     # us forward + backward, 128 / 32 queries: fp32 [80·80, 4 heads] 19 + 73 / 15 + 72, [16·256, 4] 23 + 81 / 17 + 72,
     # [64·128, 12] 37 + 152 / 45 + 163; bf16 [16·256, 4] 10 + 31 / 8 + 30, [2·2048, 8] 19 + 59 / 23 + 71.
     a.tile = 32 if S <= 64 or (fp32 and N * H * -(-S // 32) <= 1024) else 128
+    # Keys of a workgroup, dk and dv: 64 for short sequences and at fp32 (forward + backward, 128 / 64 keys, W 512:
+    # [8·2048, 8 heads] 977 / 898 us, [2·2048, 8] 336 / 280; bf16 189 / 190), but 128 at fp32 and 128 dims, where two
+    # waves would spill (1874 / 1951).
+    a.ktile = 64 if (S <= 64 or fp32) and not (fp32 and D == 128) else 128
     # The sinks' gradients from behind their window: up to 512 queries are walked by the sinks' own keys, more by a pass
     # of its own in chunks about as long as a window's walk ([80·80, 4 heads] fp32, 48 such queries: dk/dv 54 us with
     # the pass, 45 without).
@@ -197,7 +202,7 @@ def _plan(N, S, H, KV, W, sinks, scale, fp32, C, buckets, max_distance):
 
 
 def _args(q, k, v, mask, bias, cfg):
-    a = _Args.from_buffer_copy(_plan(*cfg[1:]))
+    a = _Args.from_buffer_copy(_plan(*cfg))
     a.q, a.k, a.v, a.mask, a.bias = ptr_read(q), ptr_read(k), ptr_read(v), ptr_read(mask), ptr_read(bias)
     a.ldq, a.ldk, a.ldv = q.stride(0), k.stride(0), v.stride(0)
     return a

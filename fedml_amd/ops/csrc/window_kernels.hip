@@ -519,14 +519,14 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void fwd_kernel(const Arg
 // that a column holds one distance, and a lane adds up a column and adds it to the wave's own bin of that distance;
 // blocks whose distances all lie in the last bucket are summed in registers.
 // ----------------------------------------------------------------------------------------------------------------
-template <typename T, int D, int NW, int BK, bool BIAS>
+template <typename T, int D, int NW, int BK, bool BIAS, bool DBIAS>
 __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) void dq_kernel(const Args a) {
   using R = Row<T, D>;
   __shared__ __attribute__((aligned(16))) T Ks[BK * R::P];
   __shared__ __attribute__((aligned(16))) T Vs[BK * R::P];
-  __shared__ float skew[BIAS ? NW * 2048 : 1];
+  __shared__ float skew[DBIAS ? NW * 2048 : 1];
   __shared__ float fars[NW];
-  extern __shared__ float lut[];                 // BIAS: lut, then NW × (maxd + kBinPad) bins
+  extern __shared__ float lut[];                 // BIAS: lut; DBIAS: then NW × (maxd + kBinPad) bins
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
   const typename R::Lane ln(lane);
   const int G = a.H / a.KV, nqt = (a.S + 32 * NW - 1) / (32 * NW);
@@ -544,7 +544,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
   const bool real = qi < a.S && (!mask || mask[qi]);
   const int nbin = a.maxd + kBinPad;
   float* bins = lut + lut_size(a.maxd) + w * nbin;
-  float* sk_w = skew + (BIAS ? w * 2048 : 0);
+  float* sk_w = skew + (DBIAS ? w * 2048 : 0);
   uint4 qf[R::NC], df[R::NC];
   R::frags(qf, (const T*)a.q + (tok0 + qi) * a.ldq + h * D, real, hh);
   R::frags(df, (const T*)a.dout + (tok0 + qi) * a.lddo + h * D, real, hh);
@@ -559,6 +559,8 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
   if (qi < a.S && hh == 0) a.dsum[((int64_t)n * a.H + h) * a.S + qi] = Dq;
   if (BIAS) {
     fill_lut(lut, a, n / (a.N / a.C), h, tid, 64 * NW);
+  }
+  if (DBIAS) {
     for (int i = lane; i < nbin; i += 64) bins[i] = 0.f;
     for (int i = lane; i < 2048; i += 64) sk_w[i] = 0.f;
   }
@@ -635,7 +637,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
       typename R::Cols kt;      // read ahead of ds it would cost a wave of occupancy (D 64) or spill (D 128)
       kt.read(Ks + 32 * sub * R::P, ln);
       kt.mul(acc, ds, ln);
-      if (BIAS) {
+      if (DBIAS) {
         if (near) {
           float* at = sk_w + (lane & 31) * 65 + 31 - 4 * hh;       // row i, column i − key + 31
 #pragma unroll
@@ -663,11 +665,14 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
 #pragma unroll
     for (int db = 0; db < R::DB; ++db)
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        Elem<T>::store4(out + 32 * db + 8 * c, acc[db][4 * c] * a.scale, acc[db][4 * c + 1] * a.scale,
-                        acc[db][4 * c + 2] * a.scale, acc[db][4 * c + 3] * a.scale);
+      for (int c = 0; c < 4; ++c) {
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = real ? acc[db][4 * c + j] * a.scale : 0.f;
+        Elem<T>::store4(out + 32 * db + 8 * c, x[0], x[1], x[2], x[3]);
+      }
   }
-  if (BIAS) {
+  if (DBIAS) {
     far = wave_sum(far);
     if (lane == 0) fars[w] = far;
     __syncthreads();
@@ -1173,12 +1178,11 @@ template <typename T, int D> int launch_fwd(const Args& a, hipStream_t st) {
 
 template <typename T, int D, int NW, int BK> int launch_dq(const Args& a, hipStream_t st) {
   const int64_t n = (int64_t)a.N * a.H * ((a.S + 32 * NW - 1) / (32 * NW));
-  if (a.dbias) {
-    const size_t lds = (a.maxd + 2 * kLutOff + NW * (a.maxd + kBinPad)) * sizeof(float);
-    hipLaunchKernelGGL((dq_kernel<T, D, NW, BK, true>), dim3((unsigned)n), dim3(64 * NW), lds, st, a);
-  } else {
-    hipLaunchKernelGGL((dq_kernel<T, D, NW, BK, false>), dim3((unsigned)n), dim3(64 * NW), 0, st, a);
-  }
+  const size_t lut = (a.maxd + 2 * kLutOff) * sizeof(float), bins = NW * (a.maxd + kBinPad) * sizeof(float);
+  const dim3 grid((unsigned)n), block(64 * NW);
+  if (a.dbias) hipLaunchKernelGGL((dq_kernel<T, D, NW, BK, true, true>), grid, block, lut + bins, st, a);
+  else if (a.bias) hipLaunchKernelGGL((dq_kernel<T, D, NW, BK, true, false>), grid, block, lut, st, a);
+  else hipLaunchKernelGGL((dq_kernel<T, D, NW, BK, false, false>), grid, block, 0, st, a);
   return (int)hipGetLastError();
 }
 

@@ -26,7 +26,7 @@ def half(dtype):
     return torch.finfo(dtype).eps / 2
 
 
-def _oracle(q, k, v, do, S, H, KV, window, sinks, mask, bias, M, scale, dtype):
+def _oracle(q, k, v, do, S, H, KV, window, sinks, mask, bias, M, scale, dtype, frozen=False):
     """[(value, bound)] of o, dq, dk, dv(, dbias), token-major, in 64 bits on the CPU."""
     N, D, G = q.shape[0] // S, q.shape[1] // H, H // KV
     r = half(dtype) if dtype == torch.bfloat16 else 0.0
@@ -57,7 +57,7 @@ def _oracle(q, k, v, do, S, H, KV, window, sinks, mask, bias, M, scale, dtype):
     es = torch.where(see, (D + 4) * U * a + 16 * U * (big + 1), z)
     rp = es + es.amax(-1, keepdim=True) + (n + 8) * U
     o = p @ vh
-    exact = bias is not None
+    exact = bias is not None and not frozen
     ro = r * r if exact else r
     eo = (p * (rp + ro)) @ vh.abs() + (n + 2) * U * (p @ vh.abs())
     dp, dpa = gh @ vh.mT, gh.abs() @ vh.abs().mT
@@ -249,6 +249,37 @@ def test_shared_bias_and_shared_inputs():
     assert torch.equal(o, parts[0])
     assert torch.allclose(gx, parts[1] + parts[2] + parts[3], rtol=0, atol=4 * U * 64)       # three sums of O(10)
     assert torch.allclose(gt, parts[4].sum(0), rtol=0, atol=float(parts[4].abs().sum(0).max()) * 16 * U)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("N,S", [(1, 40), (2, 150), (40, 130)])
+def test_frozen_bias_still_counts(N, S, dtype):
+    """A bias that takes no gradient is in the probabilities of every gradient; and a bias alone gets its own."""
+    H, D, window, sinks, M = 8, 64, 30, 2, 16
+    q, k, v, do = _data(N, S, H, H, D, dtype, 12)
+    bias = 2 * torch.randn(1, H, 8, generator=torch.Generator().manual_seed(3)).to(dev)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = ops.window_attention(*leaves, S, H, window, sinks, bias=bias, max_distance=M)
+    got = [o, *torch.autograd.grad(o, leaves, do)]
+    want = _oracle(q, k, v, do, S, H, H, window, sinks, None, bias, M, D ** -0.5, dtype, frozen=True)
+    for g, w, name in zip(got, want, ("o", "dq", "dk", "dv")):
+        _within(g, w, name)
+    table = bias.clone().requires_grad_()
+    o = ops.window_attention(q, k, v, S, H, window, sinks, bias=table, max_distance=M)
+    want = _oracle(q, k, v, do, S, H, H, window, sinks, None, bias, M, D ** -0.5, dtype)
+    _within(torch.autograd.grad(o, table, do)[0], want[4], "dbias")
+
+
+def test_what_a_masked_query_would_have_met():
+    """An infinite value of a real token: rows that are no token stay zero, forward and backward."""
+    N, S, H, D = 1, 70, 1, 64
+    q, k, v, do = _data(N, S, H, H, D, torch.float32, 13)
+    v[3, 5] = float("inf")
+    mask = torch.ones(N, S, dtype=torch.bool, device=dev)
+    mask[0, 40:] = False
+    got = _call((S, H, 100, 0, H, mask, 128, None), q, k, v, None, do)
+    for g in got:
+        assert not g[40:].any()
 
 
 def test_empty_batch():

@@ -10,6 +10,7 @@ CUDA tensors run the HIP kernels (bf16 or fp32 storage; states, maps and sums fp
 plain PyTorch (fp64 for fp64 inputs), the tests' oracle. Results are the same bit for bit from call to call. Everything
 is enqueued on the current stream of the tensors' device and may be captured into a HIP graph."""
 import ctypes as _c
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -45,26 +46,44 @@ def _like(x):
     return torch.empty(C, T, B, H, dtype=x.dtype, device=x.device)
 
 
-def _run(a, x, gate, mask, streams, bwd):
-    C, T, B, H = x.shape
-    a.C, a.T, a.B, a.H = C, T, B, H
-    a.x, a.gate, a.mask = ptr_read(x), ptr_read(gate), ptr_read(mask)
-    a.xs[:], a.gs[:] = x.stride()[:3], gate.stride()[:3]
-    if mask is not None:
-        a.ms[:] = mask.stride()
-    odd, es = H, x.element_size()           # two features at a time where every row starts at a multiple of two
-    for t in (x, gate, *streams):
-        s0, s1, s2, _ = t.stride()
-        odd |= s0 | s1 | s2 | t.data_ptr() // es
-    vec = 2 - (odd & 1)
+@functools.lru_cache(maxsize=512)
+def _plan(shape, xs, gs, ys, dys, ms, aligned):
+    """(what the kernels' arguments hold for all calls of these sizes and strides, features a lane takes at a time)"""
+    C, T, B, H = shape
+    a = _Args(C=C, T=T, B=B, H=H)
+    a.xs[:], a.gs[:], a.ys[:] = xs[:3], gs[:3], ys[:3]
+    odd = H
+    for st in (xs, gs, ys, dys or ()):
+        for s in st[:3]:
+            odd |= s
+    if dys is not None:
+        a.dys[:] = dys[:3]
+    if ms is not None:
+        a.ms[:] = ms
+    vec = 2 if aligned and not odd & 1 else 1       # two where every row starts at a multiple of two features
     wgs, ntile = C * B * -(-H // (32 * vec)), -(-T // _TILE)
     nseg = 1 if wgs >= _FULL else min(ntile, -(-_WANT // wgs), 64)
-    a.tps = -(-ntile // (2 * nseg)) * 2        # pairs of tiles
-    a.nseg = nseg = -(-ntile // a.tps)
-    if wgs * nseg > _I32:
+    a.tps = -(-ntile // (2 * nseg)) * 2             # pairs of tiles
+    a.nseg = -(-ntile // a.tps)
+    if wgs * a.nseg > _I32:
         raise ValueError(f"gated_scan: {C} clients · {B} sequences · {H} features are too many for one call")
-    if nseg > 1:
-        agg = torch.empty(C * B * nseg * 2 * H, dtype=torch.float32, device=x.device)
+    return a, vec
+
+
+def _run(x, gate, mask, y, h0, hT, ckpt, dy=None, dh=None, dx=None, dgate=None, dh0=None):
+    bwd = dx is not None
+    out = dx if bwd else y
+    at = x.data_ptr() | gate.data_ptr() | out.data_ptr() | (dgate.data_ptr() | dy.data_ptr() if bwd else 0)
+    plan, vec = _plan(x.shape, x.stride(), gate.stride(), out.stride(), dy.stride() if bwd else None,
+                      None if mask is None else mask.stride(), at % (2 * x.element_size()) == 0)
+    a = _Args.from_buffer_copy(plan)
+    a.x, a.gate, a.mask, a.ckpt = ptr_read(x), ptr_read(gate), ptr_read(mask), ptr_read(ckpt) if bwd else ptr(ckpt)
+    if bwd:
+        a.dy, a.dh, a.dx, a.dgate, a.dh0 = ptr_read(dy), ptr_read(dh), ptr(dx), ptr(dgate), ptr(dh0)
+    else:
+        a.y, a.hT, a.h0 = ptr(y), ptr(hT), ptr_read(h0)
+    if a.nseg > 1:
+        agg = torch.empty(a.C * a.B * a.nseg * 2 * a.H, dtype=torch.float32, device=x.device)
         a.agg = ptr(agg)
     launch("fa_gated_scan", a, (x.dtype == torch.bfloat16, vec, bwd), x.device)
 
@@ -75,10 +94,7 @@ def _forward(x, gate, h0, mask, keep):
     hT = torch.empty(C, B, H, dtype=torch.float32, device=x.device)
     ckpt = torch.empty(C, -(-T // _TILE), B, H, dtype=torch.float32, device=x.device) if keep else None
     if C * B:
-        a = _Args()
-        a.y, a.hT, a.h0, a.ckpt = ptr(y), ptr(hT), ptr_read(h0), ptr(ckpt)
-        a.ys[:] = y.stride()[:3]
-        _run(a, x, gate, mask, (y,), False)
+        _run(x, gate, mask, y, h0, hT, ckpt)
     return y, hT, ckpt
 
 
@@ -100,14 +116,10 @@ class _GatedScan(torch.autograd.Function):
         C, T, B, H = x.shape
         dy = torch.zeros_like(x) if dy is None else _dense(dy.to(x.dtype))
         dh = None if dh is None else dh.contiguous()
-        dx, dgate = _like(x), _like(x)
+        dx, dgate = _like(x), _like(x)          # of one layout
         dh0 = torch.empty(C, B, H, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
         if C * B:
-            a = _Args()
-            a.dy, a.dh, a.dx, a.dgate = ptr_read(dy), ptr_read(dh), ptr(dx), ptr(dgate)
-            a.dh0, a.ckpt = ptr(dh0), ptr_read(ckpt)
-            a.ys[:], a.dys[:] = dx.stride()[:3], dy.stride()[:3]
-            _run(a, x, gate, mask, (dx, dgate, dy), True)
+            _run(x, gate, mask, None, None, None, ckpt, dy, dh, dx, dgate, dh0)
         return dx, dgate, dh0, None
 
 

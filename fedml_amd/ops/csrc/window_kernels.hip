@@ -20,8 +20,8 @@
 // Measured on MI355X (a large copy reaches 4.94 TB/s, an 8192³ product 1420 TFLOP/s bf16 and 154 fp32):
 //   forward, bf16:  32768 tokens, 32 heads over 8, D 128, W 1024: 770 us = 714 TFLOP/s; 16 · 1999 (a quarter padding),
 //                   12 heads, D 64, W 256: 98 us
-//   dq / dk, dv:    2 · 16384, 16 heads over 4, D 128, W 1024: 520 / 1040 us = 793 / 529 TFLOP/s of the products they
-//                   make (3 and 4 a block); 16 · 1999 as above: 102 / 167 us
+//   dq / dk, dv:    2 · 16384, 16 heads over 4, D 128, W 1024: 520 / 980 us = 793 / 561 TFLOP/s of the products they
+//                   make (3 and 4 a block); 16 · 1999 as above: 102 / 157 us
 //   step, bf16:     64 caches of 4100 slots, 32 heads over 8, D 128: 225 us = 4.8 TB/s
 // A 32×32 block at D 128 takes the matrix unit 512 cycles forward, 768 in dq and 1024 in dk/dv, the vector unit about
 // 500 in each (16 exponentials a lane at a quarter rate, and what stands around them): the two share the time of a wave,
@@ -54,7 +54,7 @@ struct Args {
   const float* bias;
   int64_t ldq, ldk, ldv, lddo;
   int N, S, H, KV, C, W, sinks, NB, maxd;
-  int nchunk, qchunk;            // sink pass of the backward: chunks of queries
+  int nchunk, qchunk, nslot;     // sink pass of the backward: chunks of queries, partial sums of a kv head
   int exact;                     // forward: a gradient of the bias follows
   int tile, ktile;               // a workgroup's queries, forward and dq: 32 or 128; its keys, dk and dv: 64 or 128
   float scale;
@@ -696,7 +696,8 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
 // Backward, dk and dv: a wave owns 32 keys (its columns), the workgroup 32·NW of one kv head; it walks the queries
 // that see them through the window, for every query head of the kv head. The first workgroups are the sink pass: what
 // the sinks get from queries beyond the window, a chunk of queries each, as partial sums that finish_kernel adds up in
-// order (the sinks' own rows of the window pass among them).
+// order (the sinks' own rows of the window pass among them). There the blocks of a tile of queries go to as many waves,
+// each with the same keys and a partial sum of its own (one wave taking all: 1041 instead of 980 us at 16k tokens).
 // ----------------------------------------------------------------------------------------------------------------
 template <typename T, int D, int NW, int BQ>
 __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kernel(const Args a) {
@@ -716,7 +717,9 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
   const int kv = id % a.KV, n = id / a.KV;
   const int64_t tok0 = (int64_t)n * a.S;
   const uint8_t* mask = a.mask ? a.mask + tok0 : nullptr;
-  const int k0 = kt * 32 * NW, kw = k0 + 32 * w, kj = kw + (lane & 31);
+  constexpr int kParts = BQ / 32;
+  const int nkb = sink ? (a.sinks + 31) / 32 : NW, part = w / nkb;        // blocks of keys (sinks: ≤ 2); the wave's queries
+  const int k0 = kt * 32 * NW, kw = k0 + 32 * (w % nkb), kj = kw + (lane & 31);
   const bool real = kj < a.S && (!mask || mask[kj]) && (!sink || kj < a.sinks);
   uint4 kf[R::NC], vf[R::NC];
   R::frags(kf, (const T*)a.k + (tok0 + kj) * a.ldk + kv * D, real, hh);
@@ -769,7 +772,7 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
 #pragma unroll
     for (int sub = 0; sub < BQ / 32; ++sub) {
       const int qb = q0 + 32 * sub;
-      if (kw >= a.S || qb >= qe || qb + 31 < kw) continue;
+      if (kw >= a.S || qb >= qe || qb + 31 < kw || (sink && part != sub)) continue;
       if (sink ? (kw >= a.sinks || qb + 31 - kw < a.W) : (qb - kw - 31 >= a.W && kw >= own)) continue;
       f32x16 s = zero16(), dp = zero16();
       R::template rows2<true>(s, dp, Qs + 32 * sub * R::P, Os + 32 * sub * R::P, kf, vf, ln);
@@ -825,14 +828,14 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
   }
 #pragma unroll
   for (int db = 0; db < R::DB; ++db) settle(ak[db], av[db]);
-  if (kj >= a.S || (sink && kj >= a.sinks)) return;
+  if (kj >= a.S || (sink && (kj >= a.sinks || part >= kParts))) return;
   if (!real) {                                   // a column of no token: whatever its sums are, it has no gradient
 #pragma unroll
     for (int db = 0; db < R::DB; ++db) ak[db] = av[db] = zero16();
   }
   if (a.nchunk && kj < a.sinks) {
-    float* pk = a.part + ((((int64_t)n * a.KV + kv) * (a.nchunk + 1) + (sink ? chunk + 1 : 0)) * 2 * a.sinks + kj) * D +
-                4 * hh;
+    const int slot = sink ? 1 + chunk * kParts + part : 0;
+    float* pk = a.part + ((((int64_t)n * a.KV + kv) * a.nslot + slot) * 2 * a.sinks + kj) * D + 4 * hh;
     float* pv = pk + (int64_t)a.sinks * D;
 #pragma unroll
     for (int db = 0; db < R::DB; ++db)
@@ -886,9 +889,10 @@ __global__ __launch_bounds__(256) void finish_kernel(const Args a, int D, int nq
   if (e >= (int64_t)a.N * a.KV * one) return;
   const int64_t head = e / one;
   const int in = (int)(e % one);
-  const float4* p = reinterpret_cast<const float4*>(a.part) + head * (a.nchunk + 1) * one + in;
+  const float4* p = reinterpret_cast<const float4*>(a.part) + head * a.nslot * one + in;
   float4 s = p[0];
-  for (int i = 1; i <= a.nchunk; ++i) {
+#pragma unroll 8
+  for (int i = 1; i < a.nslot; ++i) {
     const float4 x = p[i * one];
     s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
   }

@@ -34,8 +34,8 @@ class _Args(_c.Structure):
     _fields_ = [(n, _c.c_void_p) for n in ("q", "k", "v", "dout", "o", "dq", "dk", "dv", "o32", "lse", "dsum", "part",
                                            "bpart", "dbias", "mask", "bias")] + \
                [(n, _c.c_int64) for n in ("ldq", "ldk", "ldv", "lddo")] + \
-               [(n, _c.c_int) for n in ("N", "S", "H", "KV", "C", "W", "sinks", "NB", "maxd", "nchunk", "qchunk", "exact",
-                                        "tile", "ktile")] + \
+               [(n, _c.c_int) for n in ("N", "S", "H", "KV", "C", "W", "sinks", "NB", "maxd", "nchunk", "qchunk", "nslot",
+                                        "exact", "tile", "ktile")] + \
                [("scale", _c.c_float), ("start", _c.c_int * MAX_BUCKETS)]
 
 
@@ -198,6 +198,7 @@ def _plan(D, N, S, H, KV, W, sinks, scale, fp32, C, buckets, max_distance):
     if sinks and S - W > 512:
         a.qchunk = max(512, -(-(W + 128) // 128) * 128)
         a.nchunk = -(-(S - W) // a.qchunk)
+        a.nslot = 1 + a.nchunk * (1 if fp32 else 2)      # a tile is 32 queries at fp32, two waves' 32 at bf16
     return a
 
 
@@ -252,7 +253,7 @@ class _WindowAttention(torch.autograd.Function):
             dsum = torch.empty(N, H, S, dtype=f32, device=dev)
             part = bpart = None
             if a.nchunk:
-                part = torch.empty(N, KV, a.nchunk + 1, 2, a.sinks, D, dtype=f32, device=dev)
+                part = torch.empty(N, KV, a.nslot, 2, a.sinks, D, dtype=f32, device=dev)
             if dbias is not None:
                 bpart = torch.empty(N, H, -(-S // a.tile), bias.shape[-1], dtype=f32, device=dev)
             a.dout, a.lddo, a.lse, a.o32 = ptr_read(do), do.stride(0), ptr_read(lse), ptr_read(o32)

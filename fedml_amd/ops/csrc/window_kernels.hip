@@ -495,21 +495,22 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void fwd_kernel(const Arg
   for (int db = 0; db < R::DB; ++db) settle(acc[db]);
   l = half_sum(l);
   if (qi >= a.S) return;
-  const float inv = real && l > 0.f ? 1.f / l : 0.f;
+  // A token sees itself, so l is 1 at least; l = 0 are scores that are all −inf, and 0 · (1 / 0) is the NaN that the
+  // softmax of such a row is. A NaN in l is one in every column.
+  const float inv = 1.f / l;
   const int64_t at = (tok0 + qi) * (int64_t)(a.H * D) + h * D + 4 * hh;
-  const bool nan = real && !(l >= 0.f);   // a row of non-finite scores is what the formula makes of it
 #pragma unroll
   for (int db = 0; db < R::DB; ++db)
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       float x[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = nan ? l : real ? acc[db][4 * c + j] * inv : 0.f;
+      for (int j = 0; j < 4; ++j) x[j] = real ? acc[db][4 * c + j] * inv : 0.f;
       Elem<T>::store4((T*)a.o + at + 32 * db + 8 * c, x[0], x[1], x[2], x[3]);
       if (sizeof(T) == 2 && a.o32) Elem<float>::store4(a.o32 + at + 32 * db + 8 * c, x[0], x[1], x[2], x[3]);
     }
   if (a.lse && hh == 0)
-    a.lse[((int64_t)n * a.H + h) * a.S + qi] = nan ? l : real && l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+    a.lse[((int64_t)n * a.H + h) * a.S + qi] = real ? m + __builtin_amdgcn_logf(l) : INFINITY;
 }
 
 // ----------------------------------------------------------------------------------------------------------------
@@ -1111,7 +1112,7 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 256 ? 1 : 2) void step_ker
 #pragma unroll
       for (int i = 0; i < NW; ++i)
         Lh += ml[i][1][hd] * __builtin_amdgcn_exp2f(ml[i][0][hd] - (Mh == -INFINITY ? 0.f : Mh));
-      const float inv = Lh == 0.f ? 0.f : 1.f / Lh;
+      const float inv = pos < 0 ? 0.f : 1.f / Lh;     // scores that are all −inf: 0 · (1 / 0), NaN as in fwd_kernel
       Elem<T>::store4((T*)a.o + row * D + d, s.x * inv, s.y * inv, s.z * inv, s.w * inv);
     }
   }
@@ -1135,7 +1136,7 @@ __global__ __launch_bounds__(64) void step_join_kernel(const StepArgs a) {
   for (int i = lane; i < a.splits; i += 64)
     L += a.pml[(row * a.splits + i) * 2 + 1] * __builtin_amdgcn_exp2f(a.pml[(row * a.splits + i) * 2] - Mu);
   L = wave_sum(L);
-  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const float inv = a.pos[row / a.H] < 0 ? 0.f : 1.f / L;
   for (int d = lane; d < D; d += 64) {
     float s = 0.f;
     for (int i = 0; i < a.splits; ++i)

@@ -275,7 +275,8 @@ def window_attention(q, k, v, S: int, H: int, window: int, sinks: int = 0, kv_he
     (c+1)·N/C) are client c's) is added to the scaled scores by :func:`relative_bucket_starts`' bucket of i − j.
     ``scale``: 1/√D unless given. Gradients: q, k, v (at their type) and bias (fp32).
 
-    A non-finite value in a real token's rows reaches every row that sees the token, and may reach others near it."""
+    A bias of −inf takes its bucket away; a row all of whose scores are −inf has no softmax: it is NaN, and so are the
+    gradients of what it sees. A non-finite value in a real token's rows reaches every row that sees the token, and may reach others near it."""
     D, H, KV, W, sinks = _common(q, k, v, H, kv_heads, window, sinks)
     S = int(S)
     if S < 1 or q.shape[0] % S:

@@ -130,6 +130,28 @@ def test_steps_are_the_rows_of_the_whole(window, sinks, KV):
             pos += 1
 
 
+def test_rows_of_minus_infinity_have_no_softmax():
+    """A bias of −inf takes a bucket away; a row whose every score is −inf is 0 / 0, and only it and what it sees are."""
+    S, H, M = 6, 2, 8
+    q, k, v = (t.requires_grad_() for t in _inputs(1, S, H, H, 64, 8))
+    bias = torch.zeros(H, 4, dtype=torch.float64)
+    bias[0, 0] = -math.inf                                     # no token sees itself: token 0 of head 0 sees nothing
+    bias.requires_grad_()
+    o = ops.window_attention(q, k, v, S, H, 3, bias=bias, max_distance=M)
+    assert torch.isnan(o[0, :64]).all() and torch.isfinite(o[1:]).all() and torch.isfinite(o[:, 64:]).all()
+    far = bias.detach().clone()
+    far[0, 0] = -1e4                                           # e^−10000 is 0 in 64 bits
+    assert torch.equal(o[1:], ops.window_attention(q, k, v, S, H, 3, bias=far, max_distance=M)[1:])
+    for g in torch.autograd.grad(o, (q, k, v), torch.ones_like(o)):
+        assert torch.isnan(g[0, :64]).all() and torch.isfinite(g[1:]).all() and torch.isfinite(g[:, 64:]).all()
+    kc, vc = torch.randn(2, 4, 128, dtype=torch.float64), torch.randn(2, 4, 128, dtype=torch.float64)
+    rows = [t.detach()[:2] for t in (q, k, v)]
+    all_gone = torch.full((H, 4), -math.inf, dtype=torch.float64)
+    o = ops.window_attention_step(*rows, kc, vc, torch.tensor([5, -1], dtype=torch.int32), H, 4, bias=all_gone,
+                                  max_distance=M)
+    assert torch.isnan(o[0]).all() and not o[1].any()          # an idle sequence has no row
+
+
 def test_idle_sequences_stay_as_they_are():
     kc, vc = torch.randn(3, 6, 64), torch.randn(3, 6, 64)
     before = kc.clone(), vc.clone()

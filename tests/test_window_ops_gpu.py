@@ -282,6 +282,47 @@ def test_what_a_masked_query_would_have_met():
         assert not g[40:].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("N,S,H,KV,D,window,sinks,whole", [
+    (2, 40, 2, 1, 64, 9, 0, False), (1, 300, 2, 2, 128, 70, 3, False), (1, 700, 4, 2, 64, 33, 2, True),
+    (40, 130, 8, 4, 64, 48, 0, True)])
+def test_rows_of_minus_infinity(N, S, H, KV, D, window, sinks, whole, dtype):
+    """A bias of −inf takes a bucket (or all of a head's) away. A row that keeps a key has the bits that e^−10000 gives,
+    which is 0 in 32 bits; a row that keeps none is 0 / 0, as in the CPU form, and so is all that it sees."""
+    q, k, v, do = _data(N, S, H, KV, D, dtype, 14)
+    bias = torch.randn(1, H, 8, generator=torch.Generator().manual_seed(3))
+    bias[0, 0, 0] = bias[0, H - 1, 2] = -math.inf
+    if whole:
+        bias[0, 1] = -math.inf
+    args = (S, H, window, sinks, KV, None, 32, None)
+    got = _call(args, q, k, v, bias.to(dev), do)
+    ref = _call(args, *(t.cpu().double() for t in (q, k, v)), bias.double(), do.cpu().double())
+    near = _call(args, q, k, v, bias.clamp_min(-1e4).to(dev), do)
+    for g, r, f, name in zip(got, ref, near, ("o", "dq", "dk", "dv", "dbias")):
+        nan = torch.isnan(r)
+        assert nan.any() and torch.equal(torch.isnan(g).cpu(), nan), name
+        assert torch.equal(g[~nan.to(dev)], f[~nan.to(dev)]), name
+    with torch.no_grad():
+        o = ops.window_attention(q, k, v, S, H, window, sinks, kv_heads=KV, bias=bias.to(dev), max_distance=32)
+    assert torch.equal(torch.isnan(o).cpu(), torch.isnan(ref[0]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("B,window,sinks", [(3, 9, 2), (2, 700, 4), (600, 40, 0)])
+def test_step_of_minus_infinity(B, window, sinks, dtype):
+    """The same for one token: a head whose table is all −inf gives NaN, an idle sequence's zeros stay zeros."""
+    H, D, n = 2, 64, window + sinks
+    gen = torch.Generator(device=dev).manual_seed(4)
+    q, k, v, kc, vc = (torch.randn(*s, generator=gen, device=dev).to(dtype)
+                       for s in (3 * [(B, H * D)] + 2 * [(B, n, H * D)]))
+    bias = torch.randn(H, 8, generator=gen, device=dev)
+    bias[1] = -math.inf
+    pos = torch.full((B,), n + 5, dtype=torch.int32, device=dev)
+    pos[0], pos[1] = -1, 3
+    o = ops.window_attention_step(q, k, v, kc, vc, pos, H, window, sinks, bias=bias, max_distance=32).view(B, H, D)
+    assert not o[0].any() and torch.isnan(o[1:, 1]).all() and torch.isfinite(o[1:, 0]).all()
+
+
 def test_empty_batch():
     e = torch.zeros(0, 128, device=dev, requires_grad=True)
     b = torch.zeros(1, 2, 8, device=dev, requires_grad=True)

@@ -317,6 +317,14 @@ template <typename T, int D, int ROWS, int NT> struct Stage {
   }
 };
 
+// A bias in units of log 2. The type's lowest and highest values stay finite there (those beyond 2.08e38 count as one), and
+// a product of q and k can be added to them: a row that sees nothing else than the lowest is shared out evenly.
+__device__ __forceinline__ float log2_bias(float b) {
+  const float x = b * kLog2e;
+  if (!(fabsf(b) < INFINITY)) return x;
+  return x > 3e38f ? 3e38f : x < -3e38f ? -3e38f : x;
+}
+
 // lut[d + kLutOff] = bias of distance d in units of log 2, for −94 <= d < max_distance + 94
 __device__ __forceinline__ int lut_size(int maxd) { return maxd + 2 * kLutOff; }
 __device__ __forceinline__ void fill_lut(float* lut, const Args& a, int client, int h, int tid, int nt) {
@@ -324,7 +332,7 @@ __device__ __forceinline__ void fill_lut(float* lut, const Args& a, int client, 
   for (int t = tid; t < lut_size(a.maxd); t += nt) {
     int b = 0;
     for (int i = 1; i < a.NB; ++i) b += (t - kLutOff >= a.start[i]) ? 1 : 0;
-    lut[t] = tab[b] * kLog2e;
+    lut[t] = log2_bias(tab[b]);
   }
 }
 
@@ -509,8 +517,16 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void fwd_kernel(const Arg
       Elem<T>::store4((T*)a.o + at + 32 * db + 8 * c, x[0], x[1], x[2], x[3]);
       if (sizeof(T) == 2 && a.o32) Elem<float>::store4(a.o32 + at + 32 * db + 8 * c, x[0], x[1], x[2], x[3]);
     }
-  if (a.lse && hh == 0)
-    a.lse[((int64_t)n * a.H + h) * a.S + qi] = real ? m + __builtin_amdgcn_logf(l) : INFINITY;
+  if (a.lse && hh == 0) {
+    const int64_t row = ((int64_t)n * a.H + h) * a.S + qi, all = (int64_t)a.N * a.H * a.S;
+    const float ll = __builtin_amdgcn_logf(l);
+    if (BIAS) {      // apart: next to a bias of the lowest value the logarithm would be lost
+      a.lse[row] = real ? m : 0.f;
+      a.lse[all + row] = real ? ll : INFINITY;
+    } else {
+      a.lse[row] = real ? m + ll : INFINITY;
+    }
+  }
 }
 
 // ----------------------------------------------------------------------------------------------------------------
@@ -549,12 +565,14 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
   uint4 qf[R::NC], df[R::NC];
   R::frags(qf, (const T*)a.q + (tok0 + qi) * a.ldq + h * D, real, hh);
   R::frags(df, (const T*)a.dout + (tok0 + qi) * a.lddo + h * D, real, hh);
-  float Dq = 0.f, L = INFINITY;
+  float Dq = 0.f, L = BIAS ? 0.f : INFINITY, ll = INFINITY;      // BIAS: the maximum and the sum's logarithm
   if (real) {
     const float* op = a.o32 + (tok0 + qi) * (int64_t)(a.H * D) + h * D;
 #pragma unroll
     for (int c = 0; c < R::NC; ++c) Dq = Elem<T>::dot(df[c], op + (2 * c + hh) * R::E, Dq);
-    L = a.lse[((int64_t)n * a.H + h) * a.S + qi];
+    const int64_t row = ((int64_t)n * a.H + h) * a.S + qi;
+    L = a.lse[row];
+    if (BIAS) ll = a.lse[(int64_t)a.N * a.H * a.S + row];
   }
   Dq = half_sum(Dq);
   if (qi < a.S && hh == 0) a.dsum[((int64_t)n * a.H + h) * a.S + qi] = Dq;
@@ -604,11 +622,11 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
         if (near) {
           const float* at = lut + kLutOff + qi - kb - 4 * hh;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, at[-kappa(r)] - L);
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, at[-kappa(r)]) - L - ll;
         } else {
-          const float b = lut[lut_size(a.maxd) - 1] - L;
+          const float b = lut[lut_size(a.maxd) - 1];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, b);
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c2, b) - L - ll;
         }
       } else {
 #pragma unroll
@@ -700,12 +718,12 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
 // order (the sinks' own rows of the window pass among them). There the blocks of a tile of queries go to as many waves,
 // each with the same keys and a partial sum of its own (one wave taking all: 1041 instead of 980 us at 16k tokens).
 // ----------------------------------------------------------------------------------------------------------------
-template <typename T, int D, int NW, int BQ>
+template <typename T, int D, int NW, int BQ, bool BIAS>
 __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kernel(const Args a) {
   using R = Row<T, D>;
   __shared__ __attribute__((aligned(16))) T Qs[BQ * R::P];
   __shared__ __attribute__((aligned(16))) T Os[BQ * R::P];
-  __shared__ __attribute__((aligned(16))) float Ls[BQ], Ds[BQ];
+  __shared__ __attribute__((aligned(16))) float Ls[BQ], Ds[BQ], LLs[BIAS ? BQ : 4];      // LLs: see fwd_kernel
   extern __shared__ float lut[];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5;
   const typename R::Lane ln(lane);
@@ -743,7 +761,7 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
   for (int db = 0; db < R::DB; ++db) ak[db] = av[db] = zero16();
   Stage<T, D, BQ, 64 * NW> sq, so;
   int tok = 0;
-  float sl = 0.f, sd = 0.f;                        // threads below BQ: the row's statistics
+  float sl = 0.f, sd = 0.f, sll = 0.f;             // threads below BQ: the row's statistics
   auto load = [&](int it) {
     const int h = kv * G + it / nt, q0 = qs + (it % nt) * BQ;
     tok = token<BQ>(mask, q0, qe, lane);
@@ -751,7 +769,8 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
     so.load((const T*)a.dout + tok0 * a.lddo + h * D, a.lddo, q0, qe - 1, tid);
     if (tid < BQ) {
       const int64_t at = ((int64_t)n * a.H + h) * a.S + q0 + tid;
-      sl = q0 + tid < qe ? a.lse[at] : INFINITY;   // a masked query's is +inf, its D zero
+      sl = q0 + tid < qe ? a.lse[at] : BIAS ? 0.f : INFINITY;      // a masked query's (sum) is +inf, its D zero
+      if (BIAS) sll = q0 + tid < qe ? a.lse[(int64_t)a.N * a.H * a.S + at] : INFINITY;
       sd = q0 + tid < qe ? a.dsum[at] : 0.f;
     }
   };
@@ -764,9 +783,10 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
     so.store(Os, bits, tid);
     if (tid < BQ) {
       Ls[tid] = sl;
+      if (BIAS) LLs[tid] = sll;
       Ds[tid] = sd;
     }
-    if (a.bias && it % nt == 0) fill_lut(lut, a, n / (a.N / a.C), kv * G + it / nt, tid, 64 * NW);
+    if (BIAS && it % nt == 0) fill_lut(lut, a, n / (a.N / a.C), kv * G + it / nt, tid, 64 * NW);
     __syncthreads();
     if (it + 1 < count) load(it + 1);
     const bool whole = sink ? q0 - kw - 31 >= a.W : q0 >= kw + 31 && (q0 + BQ - 1 - kw < a.W || kw + 31 < own);
@@ -779,7 +799,7 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
       R::template rows2<true>(s, dp, Qs + 32 * sub * R::P, Os + 32 * sub * R::P, kf, vf, ln);
       typename R::Cols ot, qt;
       ot.read(Os + 32 * sub * R::P, ln);
-      if (a.bias) {
+      if (BIAS) {
         if (qb - kw - 31 < a.maxd) {
           const float* at = lut + kLutOff + qb - kj + 4 * hh;
 #pragma unroll
@@ -796,10 +816,15 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
         const float4 L4 = *reinterpret_cast<const float4*>(Ls + 32 * sub + 8 * c + 4 * hh);
         const float4 D4 = *reinterpret_cast<const float4*>(Ds + 32 * sub + 8 * c + 4 * hh);
         const float Lr[4] = {L4.x, L4.y, L4.z, L4.w}, Dr[4] = {D4.x, D4.y, D4.z, D4.w};
+        float ll[4] = {0.f, 0.f, 0.f, 0.f};
+        if (BIAS) {
+          const float4 x = *reinterpret_cast<const float4*>(LLs + 32 * sub + 8 * c + 4 * hh);
+          ll[0] = x.x; ll[1] = x.y; ll[2] = x.z; ll[3] = x.w;
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = 4 * c + j;
-          p[r] = __builtin_amdgcn_exp2f(a.bias ? s[r] - Lr[j] : fmaf(s[r], c2, -Lr[j]));
+          p[r] = __builtin_amdgcn_exp2f(BIAS ? s[r] - Lr[j] - ll[j] : fmaf(s[r], c2, -Lr[j]));
           ds[r] = p[r] * (dp[r] - Dr[j]);
         }
       }
@@ -955,7 +980,7 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 256 ? 1 : 2) void step_ker
   if (a.bias) {
     const float* src = a.bias + ((int64_t)(b / (a.B / a.C)) * a.H + kv * G + grp * 32) * a.NB;
     const int have = (G - grp * 32 < 32 ? G - grp * 32 : 32) * a.NB;
-    for (int i = tid; i < 32 * a.NB; i += 64 * NW) tab[i] = i < have ? src[i] * kLog2e : 0.f;
+    for (int i = tid; i < 32 * a.NB; i += 64 * NW) tab[i] = i < have ? log2_bias(src[i]) : 0.f;
     for (int d = tid; d <= a.maxd; d += 64 * NW) {
       int x = 0;
       for (int i = 1; i < a.NB; ++i) x += d >= a.start[i] ? 1 : 0;
@@ -1200,9 +1225,12 @@ template <typename T, int D> int launch_bwd(const Args& a, hipStream_t st) {
   const int64_t nsink = (int64_t)a.nchunk * a.N * a.KV;
   const int64_t n = nsink + (int64_t)a.N * a.KV * ((a.S + a.ktile - 1) / a.ktile);
   if (a.ktile == 128) {
-    hipLaunchKernelGGL((dkv_kernel<T, D, 4, sizeof(T) == 2 ? 64 : 32>), dim3((unsigned)n), dim3(256), lds, st, a);
+    constexpr int BQ = sizeof(T) == 2 ? 64 : 32;
+    if (a.bias) hipLaunchKernelGGL((dkv_kernel<T, D, 4, BQ, true>), dim3((unsigned)n), dim3(256), lds, st, a);
+    else hipLaunchKernelGGL((dkv_kernel<T, D, 4, BQ, false>), dim3((unsigned)n), dim3(256), 0, st, a);
   } else if constexpr (D * sizeof(T) <= 256) {
-    hipLaunchKernelGGL((dkv_kernel<T, D, 2, 32>), dim3((unsigned)n), dim3(128), lds, st, a);
+    if (a.bias) hipLaunchKernelGGL((dkv_kernel<T, D, 2, 32, true>), dim3((unsigned)n), dim3(128), lds, st, a);
+    else hipLaunchKernelGGL((dkv_kernel<T, D, 2, 32, false>), dim3((unsigned)n), dim3(128), 0, st, a);
   } else {
     return (int)hipErrorInvalidValue;
   }

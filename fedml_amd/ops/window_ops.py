@@ -217,7 +217,8 @@ def _forward(q, k, v, mask, bias, cfg, keep, exact):
     o32 = lse = None
     if keep:
         o32 = torch.empty(N * S, H * D, dtype=torch.float32, device=dev) if bf16 else o
-        lse = torch.empty(N, H, S, dtype=torch.float32, device=dev)
+        # log-sum-exp; with a bias the maximum and the logarithm of the sum
+        lse = torch.empty(1 if bias is None else 2, N, H, S, dtype=torch.float32, device=dev)
     if N:
         a = _args(q, k, v, mask, bias, cfg)
         a.o, a.o32, a.lse, a.exact = ptr(o), ptr(o32), ptr(lse), exact
@@ -275,7 +276,7 @@ def window_attention(q, k, v, S: int, H: int, window: int, sinks: int = 0, kv_he
     (c+1)·N/C) are client c's) is added to the scaled scores by :func:`relative_bucket_starts`' bucket of i − j.
     ``scale``: 1/√D unless given. Gradients: q, k, v (at their type) and bias (fp32).
 
-    A bias of −inf takes its bucket away; a row all of whose scores are −inf has no softmax: it is NaN, and so are the
+    Biases beyond ±2.08e38 count as one. A bias of −inf takes its bucket away; a row all of whose scores are −inf has no softmax: it is NaN, and so are the
     gradients of what it sees. A non-finite value in a real token's rows reaches every row that sees the token, and may reach others near it."""
     D, H, KV, W, sinks = _common(q, k, v, H, kv_heads, window, sinks)
     S = int(S)

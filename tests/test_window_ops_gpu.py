@@ -323,6 +323,49 @@ def test_step_of_minus_infinity(B, window, sinks, dtype):
     assert not o[0].any() and torch.isnan(o[1:, 1]).all() and torch.isfinite(o[1:, 0]).all()
 
 
+def _apart(N, S, H, KV, D, dtype, seed):
+    """Inputs whose scores are all exactly zero: queries and keys share no dim."""
+    q, k, v, do = _data(N, S, H, KV, D, dtype, seed)
+    q.view(N * S, H, D)[..., D // 2:] = 0
+    k.view(N * S, KV, D)[..., :D // 2] = 0
+    return q, k, v, do
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("N,S,H,KV,D,window,sinks,maxd", [
+    (2, 40, 2, 1, 64, 9, 0, 32), (1, 300, 3, 3, 128, 70, 3, 32), (1, 700, 4, 2, 64, 33, 2, 16),
+    (40, 130, 8, 4, 64, 48, 0, 32)])
+def test_bias_of_the_lowest_and_highest_value(N, S, H, KV, D, window, sinks, maxd, dtype):
+    """A table with the type's lowest value: a row that sees nothing else is shared out evenly, forward and backward (a
+    score's few units are nothing to it: here they are zero). −200 is the same in 64 bits, up to e^−200. The highest
+    value, in a bucket of the third head, takes all of a row that sees it, as 200 does."""
+    q, k, v, do = _apart(N, S, H, KV, D, dtype, 15)
+    low = torch.zeros(1, H, 8)
+    low[0, 0, :3] = low[0, 1] = -200.0
+    if H > 2:
+        low[0, 2, 3] = 200.0
+    top = torch.finfo(torch.float32).max
+    bias = torch.where(low < 0, -top, torch.where(low > 0, top, 0.0))
+    got = _call((S, H, window, sinks, KV, None, maxd, None), q, k, v, bias.to(dev), do)
+    want = _oracle(q, k, v, do, S, H, KV, window, sinks, None, low, maxd, D ** -0.5, dtype)
+    for g, w, name in zip(got, want, ("o", "dq", "dk", "dv", "dbias")):
+        _within(g, w, name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("B,window,sinks", [(3, 9, 2), (2, 700, 4), (600, 40, 0)])
+def test_step_bias_of_the_lowest_value(B, window, sinks, dtype):
+    H, D, n = 2, 64, window + sinks
+    q, k, v, _ = _apart(B, 1, H, H, D, dtype, 16)
+    kc, vc = (t.view(B, n, H * D) for t in _apart(B, n, H, H, D, dtype, 17)[1:3])
+    low = torch.zeros(H, 8, device=dev)
+    low[0, :3] = low[1] = -200.0
+    pos = (torch.arange(B, device=dev) * 7 % (2 * n)).to(torch.int32)
+    o = ops.window_attention_step(q, k, v, kc, vc, pos, H, window, sinks, max_distance=32,
+                                  bias=torch.where(low < 0, torch.finfo(torch.float32).min, low))
+    _within(o, _step_bound(q, kc, vc, pos, H, H, window, sinks, low.unsqueeze(0), 32, D ** -0.5, dtype), "o")
+
+
 def test_empty_batch():
     e = torch.zeros(0, 128, device=dev, requires_grad=True)
     b = torch.zeros(1, 2, 8, device=dev, requires_grad=True)

@@ -584,6 +584,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
     for (int i = lane; i < 2048; i += 64) sk_w[i] = 0.f;
   }
   float far = 0.f;
+  const bool all_real = __all(real);
   const KeyTiles tiles(a, q0, 32 * NW, BK);
   const int count = __syncthreads_or(real) ? tiles.count : 0;
   const float c2 = a.scale * kLog2e;
@@ -652,6 +653,10 @@ __global__ __launch_bounds__(64 * NW, NW == 1 || D * sizeof(T) > 256 ? 1 : 2) vo
         const uint32_t mine = (uint32_t)(bits >> (32 * sub)) >> (4 * hh);
 #pragma unroll
         for (int r = 0; r < 16; ++r) ds[r] = (mine >> kappa(r)) & 1 ? ds[r] : 0.f;
+      }
+      if (DBIAS && !all_real) {      // e^−inf is 0, but for a bias that is not finite where only padding looks
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] = real ? ds[r] : 0.f;
       }
       typename R::Cols kt;      // read ahead of ds it would cost a wave of occupancy (D 64) or spill (D 128)
       kt.read(Ks + 32 * sub * R::P, ln);
@@ -845,6 +850,14 @@ __global__ __launch_bounds__(64 * NW, D * sizeof(T) > 128 ? 1 : 2) void dkv_kern
             p[r] = see ? p[r] : 0.f;
             ds[r] = see ? ds[r] : 0.f;
           }
+        }
+      }
+      if (BIAS && bits != ~0ull >> (64 - BQ)) {      // queries that are no token, as in dq_kernel
+        const uint32_t mine = (uint32_t)(bits >> (32 * sub)) >> (4 * hh);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          p[r] = (mine >> kappa(r)) & 1 ? p[r] : 0.f;
+          ds[r] = (mine >> kappa(r)) & 1 ? ds[r] : 0.f;
         }
       }
       qt.read(Qs + 32 * sub * R::P, ln);

@@ -366,6 +366,24 @@ def test_step_bias_of_the_lowest_value(B, window, sinks, dtype):
     _within(o, _step_bound(q, kc, vc, pos, H, H, window, sinks, low.unsqueeze(0), 32, D ** -0.5, dtype), "o")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("S,window,sinks", [(60, 60, 0), (150, 100, 4), (1200, 90, 3)])
+def test_buckets_that_only_padding_reaches(S, window, sinks, dtype):
+    """What a table holds for distances that no two tokens are apart reaches no gradient, as it reaches no output."""
+    N, H, KV, D = 3, 4, 2, 64
+    q, k, v, do = _data(N, S, H, KV, D, dtype, 18)
+    mask = torch.arange(S, device=dev) < torch.tensor([[15], [9], [0]], device=dev)
+    bias = torch.randn(1, H, 8, generator=torch.Generator().manual_seed(3)).to(dev)
+    assert ops.relative_bucket_starts(8, 64)[6] > 14       # buckets 6 and 7 begin behind the longest sequence
+    bias[..., 6:] = 0.0
+    want = _call((S, H, window, sinks, KV, mask, 64, None), q, k, v, bias, do)
+    for fill in (float("nan"), float("inf")):
+        bias[..., 6:] = fill
+        got = _call((S, H, window, sinks, KV, mask, 64, None), q, k, v, bias, do)
+        for g, w, name in zip(got, want, ("o", "dq", "dk", "dv", "dbias")):
+            assert torch.equal(g, w), name
+
+
 def test_empty_batch():
     e = torch.zeros(0, 128, device=dev, requires_grad=True)
     b = torch.zeros(1, 2, 8, device=dev, requires_grad=True)

@@ -96,6 +96,8 @@ def _common(q, k, v, H, kv_heads, window, sinks):
     D = _rows(q, H, "q")
     if D not in (64, 128):
         raise ValueError(f"head dim 64 or 128 expected, got {D}")
+    if q.shape[1] > _I32:                        # the kernels' offsets inside a row are 32 bits wide
+        raise ValueError(f"{H} heads of dim {D}: at most 2^31 − 1 elements a row")
     for t, n in ((k, "k"), (v, "v")):
         if _rows(t, KV, n, q.shape[0], q.dtype, q.device) != D:
             raise ValueError(f"{n}: {KV} heads of dim {D} expected, got {tuple(t.shape)}")

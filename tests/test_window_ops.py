@@ -196,6 +196,18 @@ def test_refusals(error, match, kw):
         ops.window_attention(**a)
 
 
+def test_rows_past_32_bits_are_refused():
+    H = 2 ** 31 // 64
+    row = torch.zeros(1, 1).expand(1, H * 64)                  # no memory behind it
+    for KV in (1, H):
+        kv = row[:, :KV * 64]
+        with pytest.raises(ValueError, match="elements a row"):
+            ops.window_attention(row, kv, kv, 1, H, 1, kv_heads=KV)
+        with pytest.raises(ValueError, match="elements a row"):
+            ops.window_attention_step(row, kv, kv, *(torch.zeros(1).expand(1, 1, KV * 64) for _ in range(2)),
+                                      torch.zeros(1, dtype=torch.int32), H, 1, kv_heads=KV)
+
+
 @pytest.mark.parametrize("error,match,kw", [
     (ValueError, "k_cache", dict(k_cache=_t(2, 4, 128))), (ValueError, "v_cache", dict(v_cache=_t(2, 5, 64))),
     (ValueError, "v_cache", dict(v_cache=_t(2, 5, 128, dtype=torch.bfloat16))),

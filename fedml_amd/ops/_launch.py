@@ -6,6 +6,8 @@ import torch
 
 from . import fl_ops
 
+MAX_THREADS = 2 ** 32 - 1        # of a launch: workgroups · threads of a workgroup
+
 
 def ptr(t):
     """Address of an operand the kernel writes (None: null)."""

@@ -15,7 +15,7 @@ import functools
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._launch import launch, ptr, ptr_read
+from ._launch import MAX_THREADS, launch, ptr, ptr_read
 from .fl_ops import use_native
 
 _TILE = 32                # steps between two kept states
@@ -65,7 +65,7 @@ def _plan(shape, xs, gs, ys, dys, ms, aligned):
     nseg = 1 if wgs >= _FULL else min(ntile, -(-_WANT // wgs), 64)
     a.tps = -(-ntile // (2 * nseg)) * 2             # pairs of tiles
     a.nseg = -(-ntile // a.tps)
-    if wgs * a.nseg > _I32:
+    if 256 * wgs * a.nseg > MAX_THREADS:
         raise ValueError(f"gated_scan: {C} clients · {B} sequences · {H} features are too many for one call")
     return a, vec
 

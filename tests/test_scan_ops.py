@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from fedml_amd import ops
+from fedml_amd.ops import scan_ops
 
 
 def _inputs(C, T, B, H, seed=0):
@@ -69,6 +70,21 @@ def test_padding_reaches_nothing():
     gy[~mask] = float("nan")
     for g in torch.autograd.grad((y, hT), bad, (gy, torch.ones_like(hT))):
         assert torch.isfinite(g).all() and not g[~mask].any()
+
+
+@pytest.mark.parametrize("C,T,B,H,pair", [(1, 1, 2 ** 24, 1, False), (4, 1, 2 ** 22, 2, True), (2, 5, 1, 2 ** 28, False),
+                                          (1, 1, 1, 2 ** 30, True)])
+def test_calls_that_no_launch_holds_are_refused(C, T, B, H, pair):
+    """A launch has fewer than 2^32 threads: 2^24 − 1 workgroups of 256, one for 32 features of a sequence (64 in pairs)."""
+    strides = (T * B * H, B * H, H, 1)
+
+    def plan(b, h):
+        return scan_ops._plan((C, T, b, h), strides, strides, strides, None, None, pair)
+
+    with pytest.raises(ValueError, match="too many"):
+        plan(B, H)
+    a, vec = plan(*((B - 1, H) if B > 1 else (B, H - 128)))
+    assert C * a.B * -(-a.H // (32 * vec)) * a.nseg * 256 < 2 ** 32
 
 
 def _t(*shape, dtype=torch.float32):

@@ -21,7 +21,7 @@ import math
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._launch import launch, ptr, ptr_read
+from ._launch import MAX_THREADS, launch, ptr, ptr_read
 from .fl_ops import _check, _fn, _i64, _p, _pr, _stream, use_native
 
 MAX_SINKS = 64
@@ -179,8 +179,8 @@ def _window_ref(q, k, v, S, H, KV, W, sinks, mask, bias, max_distance, scale):
 
 # --------------------------------------------------------------------------------------------------------- training
 @functools.lru_cache(maxsize=256)
-def _plan(D, N, S, H, KV, W, sinks, scale, fp32, C, buckets, max_distance):
-    """What the kernels' arguments hold for all calls of these sizes."""
+def _plan(D, N, S, H, KV, W, sinks, scale, fp32, C, buckets, max_distance, train):
+    """What the kernels' arguments hold for all calls of these sizes (train: with a backward pass)."""
     a = _Args(N=N, S=S, H=H, KV=KV, C=C, W=W, sinks=sinks, NB=buckets, scale=scale)
     if buckets:
         a.maxd = max_distance
@@ -201,6 +201,13 @@ def _plan(D, N, S, H, KV, W, sinks, scale, fp32, C, buckets, max_distance):
         a.qchunk = max(512, -(-(W + 128) // 128) * 128)
         a.nchunk = -(-(S - W) // a.qchunk)
         a.nslot = 1 + a.nchunk * (1 if fp32 else 2)      # a tile is 32 queries at fp32, two waves' 32 at bf16
+    # a wave for 32 queries or keys of a head; finish_kernel: a thread for 4 columns of a sink's two gradients
+    threads = [2 * N * H * -(-S // a.tile) * a.tile]
+    if train:
+        threads += [2 * N * KV * (a.nchunk + -(-S // a.ktile)) * a.ktile,
+                    256 * C * H + (N * KV * sinks * D // 2 + 255 if a.nchunk else 0)]
+    if max(threads) > MAX_THREADS:
+        raise ValueError(f"{N} sequences · {H} heads · {S} tokens are too many for one call")
     return a
 
 
@@ -278,8 +285,9 @@ def window_attention(q, k, v, S: int, H: int, window: int, sinks: int = 0, kv_he
     (c+1)·N/C) are client c's) is added to the scaled scores by :func:`relative_bucket_starts`' bucket of i − j.
     ``scale``: 1/√D unless given. Gradients: q, k, v (at their type) and bias (fp32).
 
-    Biases beyond ±2.08e38 count as one. A bias of −inf takes its bucket away; a row all of whose scores are −inf has no softmax: it is NaN, and so are the
-    gradients of what it sees. A non-finite value in a real token's rows reaches every row that sees the token, and may reach others near it."""
+    Biases beyond ±2.08e38 count as one. A bias of −inf takes its bucket away; a row all of whose scores are −inf has no
+    softmax: it is NaN, and so are the gradients of what it sees. A non-finite value in a real token's rows reaches
+    every row that sees the token, and may reach others near it."""
     D, H, KV, W, sinks = _common(q, k, v, H, kv_heads, window, sinks)
     S = int(S)
     if S < 1 or q.shape[0] % S:
@@ -297,10 +305,11 @@ def window_attention(q, k, v, S: int, H: int, window: int, sinks: int = 0, kv_he
         return _window_ref(q, k, v, S, H, KV, W, sinks, mask, table, max_distance, scale)
     if mask is not None:
         mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous().view(torch.uint8)
+    train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                         (table is not None and table.requires_grad))
     cfg = (D, N, S, H, KV, min(W, S), min(sinks, S), scale, q.dtype == torch.float32,
-           *((0, 0, 0) if table is None else (table.shape[0], table.shape[2], int(max_distance))))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
-                                    (table is not None and table.requires_grad)):
+           *((0, 0, 0) if table is None else (table.shape[0], table.shape[2], int(max_distance))), train)
+    if train:
         return _WindowAttention.apply(q, k, v, table, mask, cfg)
     tab = None if table is None else table.contiguous()
     return _forward(_aligned(q), _aligned(k), _aligned(v), mask, tab, cfg, False, False)[0]
@@ -357,14 +366,14 @@ def _step_ref(q, k, v, kc, vc, pos, H, KV, W, sinks, bias, max_distance, scale):
 
 
 @functools.lru_cache(maxsize=256)
-def _step_plan(B, H, KV, W, sinks, scale, C, buckets, max_distance):
+def _step_plan(B, H, KV, W, sinks, scale, threads, C, buckets, max_distance):
     # enough workgroups for 256 CUs, of at least one 32-slot tile a wave
     n, wgs = W + sinks, B * KV * -(-(H // KV) // 32)
     tiles = -(-n // 128)
     splits = max(1, min(tiles, -(-512 // wgs)))
     per = -(-tiles // splits) * 128
     splits = -(-n // per)
-    if wgs * splits > _I32 or B * H > _I32 or n > 2 ** 30:
+    if threads * wgs * splits > MAX_THREADS or B * H > _I32 or n > 2 ** 30:
         raise ValueError(f"{B} sequences of {H} heads and {n} slots are too many for one call")
     a = _StepArgs(B=B, H=H, KV=KV, C=C, W=W, sinks=sinks, NB=buckets, splits=splits, per=per, scale=scale)
     if buckets:
@@ -397,7 +406,8 @@ def window_attention_step(q, k, v, k_cache, v_cache, pos, H: int, window: int, s
         return o
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
     tab = None if table is None else table.contiguous()
-    plan = _step_plan(B, H, KV, W, sinks, scale, *((1, 0, 0) if tab is None else
+    threads = 128 if D == 128 and q.dtype == torch.float32 else 256
+    plan = _step_plan(B, H, KV, W, sinks, scale, threads, *((1, 0, 0) if tab is None else
                                                    (tab.shape[0], tab.shape[2], int(max_distance))))
     a = _StepArgs.from_buffer_copy(plan)
     a.q, a.k, a.v, a.kc, a.vc = ptr_read(q), ptr_read(k), ptr_read(v), ptr(k_cache), ptr(v_cache)

@@ -208,6 +208,32 @@ def test_rows_past_32_bits_are_refused():
                                       torch.zeros(1, dtype=torch.int32), H, 1, kv_heads=KV)
 
 
+@pytest.mark.parametrize("N,S,H,KV,sinks,train,ok", [
+    (2 ** 26 - 1, 1, 1, 1, 0, False, True), (2 ** 26, 1, 1, 1, 0, False, False),      # 64 threads a row of one token
+    (2 ** 25 - 1, 1, 1, 1, 0, True, True), (2 ** 25, 1, 1, 1, 0, True, False),        # dk/dv: 128
+    (2 ** 25, 1, 2, 1, 0, False, False), (2 ** 24 - 1, 65, 1, 1, 0, False, True), (2 ** 24, 65, 1, 1, 0, False, False),
+    (2 ** 20, 64, 1, 1, 64, True, True), (2 ** 21, 1000, 1, 1, 64, True, False)])
+def test_calls_that_no_launch_holds_are_refused(N, S, H, KV, sinks, train, ok):
+    """A launch has fewer than 2^32 threads."""
+    def plan():
+        return W._plan(64, N, S, H, KV, min(64, S), min(sinks, S), 0.125, False, 0, 0, 0, train)
+    if not ok:
+        with pytest.raises(ValueError, match="too many"):
+            plan()
+        return
+    a = plan()
+    assert 2 * a.tile * N * H * -(-S // a.tile) < 2 ** 32
+    assert not train or 2 * a.ktile * N * KV * (a.nchunk + -(-S // a.ktile)) < 2 ** 32
+
+
+def test_steps_that_no_launch_holds_are_refused():
+    for threads in (128, 256):
+        most = (2 ** 32 - 1) // threads
+        assert W._step_plan(most, 1, 1, 5, 1, 0.125, threads, 1, 0, 0).splits == 1
+        with pytest.raises(ValueError, match="too many"):
+            W._step_plan(most + 1, 1, 1, 5, 1, 0.125, threads, 1, 0, 0)
+
+
 @pytest.mark.parametrize("error,match,kw", [
     (ValueError, "k_cache", dict(k_cache=_t(2, 4, 128))), (ValueError, "v_cache", dict(v_cache=_t(2, 5, 64))),
     (ValueError, "v_cache", dict(v_cache=_t(2, 5, 128, dtype=torch.bfloat16))),

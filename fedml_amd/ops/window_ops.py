@@ -129,8 +129,8 @@ def _bias(bias, sequences, H, max_distance, device):
 
 def _scale(scale, D):
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"scale > 0 expected, got {scale}")
+    if not 2.0 ** -126 <= scale <= 2.0 ** 127:      # in fp32, and with log2 e, neither zero nor infinite
+        raise ValueError(f"scale in [2^-126, 2^127] expected, got {scale}")
     return scale
 
 

@@ -196,6 +196,18 @@ def test_refusals(error, match, kw):
         ops.window_attention(**a)
 
 
+@pytest.mark.parametrize("scale", [1e-60, 2.0 ** -127, 2.0 ** 128, 3e38, 1e300, math.inf, -0.1])
+def test_scales_that_32_bits_do_not_hold_are_refused(scale):
+    q = torch.ones(4, 64)
+    with pytest.raises(ValueError, match="scale"):
+        ops.window_attention(q, q, q, 4, 1, 3, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        ops.window_attention_step(q, q, q, _t(4, 3, 64), _t(4, 3, 64), torch.zeros(4, dtype=torch.int32), 1, 3,
+                                  scale=scale)
+    for fine in (2.0 ** -126, 2.0 ** 127):
+        ops.window_attention(q * 0, q, q, 4, 1, 3, scale=fine)
+
+
 def test_rows_past_32_bits_are_refused():
     H = 2 ** 31 // 64
     row = torch.zeros(1, 1).expand(1, H * 64)                  # no memory behind it

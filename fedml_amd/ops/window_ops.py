@@ -325,8 +325,18 @@ def _cache(k_cache, v_cache, B, KV, D, slots, dtype, device):
             raise ValueError(f"{n}: contiguous, 16-byte aligned memory expected (it is updated in place)")
         if t.requires_grad:
             raise ValueError(f"{n} takes no gradient")
-    if k_cache.numel() and k_cache.data_ptr() == v_cache.data_ptr():
+    size = k_cache.numel() * k_cache.element_size()
+    if abs(k_cache.data_ptr() - v_cache.data_ptr()) < size:
         raise ValueError("k_cache and v_cache are the same memory")
+    return k_cache.data_ptr(), v_cache.data_ptr(), size
+
+
+def _apart(t, caches):
+    """The rows, or a copy of rows that lie in a cache, which the call writes while it reads them."""
+    lo = t.data_ptr()
+    hi = lo + ((t.shape[0] - 1) * t.stride(0) + (t.shape[1] - 1) * t.stride(1) + 1) * t.element_size()
+    k, v, size = caches
+    return t.clone() if (lo < k + size and hi > k) or (lo < v + size and hi > v) else t
 
 
 def _pos(pos, B, device, name):
@@ -392,18 +402,19 @@ def window_attention_step(q, k, v, k_cache, v_cache, pos, H: int, window: int, s
     caller counts ``pos`` on, once per token for all layers; no gradient."""
     D, H, KV, W, sinks = _common(q, k, v, H, kv_heads, window, sinks)
     B, n = q.shape[0], W + sinks
-    _cache(k_cache, v_cache, B, KV, D, n, q.dtype, q.device)
+    caches = _cache(k_cache, v_cache, B, KV, D, n, q.dtype, q.device)
     pos = _pos(pos, B, q.device, "pos")
     table = _bias(bias, B, H, max_distance, q.device)
     scale = _scale(scale, D)
     if (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)) and \
             torch.is_grad_enabled():
         raise ValueError("window_attention_step computes no gradient: call it under torch.no_grad()")
+    if B == 0:
+        return torch.empty(B, H * D, dtype=q.dtype, device=q.device)
+    q, k, v = _apart(q, caches), _apart(k, caches), _apart(v, caches)
     if not use_native(q):
         return _step_ref(q, k, v, k_cache, v_cache, pos, H, KV, W, sinks, table, max_distance, scale)
     o = torch.empty(B, H * D, dtype=q.dtype, device=q.device)
-    if B == 0:
-        return o
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
     tab = None if table is None else table.contiguous()
     threads = 128 if D == 128 and q.dtype == torch.float32 else 256
@@ -434,18 +445,19 @@ def window_cache_fill(k, v, S: int, k_cache, v_cache, window: int, sinks: int = 
         _rows(t, 1, n, B * S, k_cache.dtype, k_cache.device)
         if t.shape[1] != width or width % 64:
             raise ValueError(f"{n}: rows of the cache's {width} columns expected, got {t.shape[1]}")
-    _cache(k_cache, v_cache, B, 1, width, W + sinks, k.dtype, k.device)
+    caches = _cache(k_cache, v_cache, B, 1, width, W + sinks, k.dtype, k.device)
     if lengths is not None:
         lengths = _pos(lengths, B, k.device, "lengths")
+    if B == 0:
+        return
     with torch.no_grad():
+        k, v = _apart(k, caches), _apart(v, caches)
         if not use_native(k):
             last = (torch.full((B,), S, device=k.device) if lengths is None else lengths.clamp(0, S)) - 1
             tok = _slot_tokens(last, W + sinks, W, sinks)
             at = tok.clamp_min(0) + torch.arange(B, device=k.device).view(B, 1) * S
             for t, c in ((k, k_cache), (v, v_cache)):
                 c.copy_(torch.where((tok >= 0).unsqueeze(-1), t[at], c))
-            return
-        if B == 0:
             return
         k, v = _aligned(k), _aligned(v)
         e = 16 // k.element_size()

@@ -196,6 +196,33 @@ def test_refusals(error, match, kw):
         ops.window_attention(**a)
 
 
+def test_caches_that_overlap_are_refused():
+    buf = _t(3, 5, 128)
+    row, pos = _t(2, 128), torch.zeros(2, dtype=torch.int32)
+    for a, b in ((buf[:2], buf[1:]), (buf[1:], buf[:2]), (buf[:2], buf[:2])):
+        with pytest.raises(ValueError, match="same memory"):
+            ops.window_attention_step(row, row, row, a, b, pos, 2, 4, 1)
+        with pytest.raises(ValueError, match="same memory"):
+            ops.window_cache_fill(_t(6, 128), _t(6, 128), 3, a, b, 4, 1)
+    both = _t(4, 5, 128)                                       # two caches of one piece of memory
+    ops.window_attention_step(row, row, row, both[:2], both[2:], pos, 2, 4, 1)
+
+
+def test_rows_that_lie_in_a_cache():
+    """Rows of the caches as arguments: what they held before the call counts."""
+    both = torch.randn(2, 2, 5, 128, generator=torch.Generator().manual_seed(9))
+    pos = torch.tensor([3, 8], dtype=torch.int32)              # slots 3 and 4
+    for pick in (lambda c: (c[0, :, 3], c[1, :, 3], c[0, :, 4]), lambda c: (c[1, :, 4], c[1, :, 3], c[0, :, 3])):
+        mine, ref = both.clone(), both.clone()
+        o = ops.window_attention_step(*pick(mine), *mine, pos, 2, 4, 1)
+        want = ops.window_attention_step(*(t.clone() for t in pick(both)), *ref, pos, 2, 4, 1)
+        assert torch.equal(o, want) and torch.equal(mine, ref)
+    mine, ref = both.clone(), both.clone()
+    ops.window_cache_fill(mine[1].view(10, 128), mine[0].view(10, 128), 5, *mine, 4, 1)
+    ops.window_cache_fill(both[1].reshape(10, 128).clone(), both[0].reshape(10, 128).clone(), 5, *ref, 4, 1)
+    assert torch.equal(mine, ref)
+
+
 @pytest.mark.parametrize("scale", [1e-60, 2.0 ** -127, 2.0 ** 128, 3e38, 1e300, math.inf, -0.1])
 def test_scales_that_32_bits_do_not_hold_are_refused(scale):
     q = torch.ones(4, 64)

@@ -518,6 +518,23 @@ def test_fill(S, window, sinks, dtype):
         assert all(torch.equal(c.cpu(), w) for c, w in zip(caches, want))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_rows_that_lie_in_a_cache(dtype):
+    """Rows of the caches as arguments: what they held before the call counts."""
+    B, n, H, D = 40, 69, 2, 64
+    both = torch.randn(2, B, n, H * D, generator=torch.Generator(device=dev).manual_seed(9), device=dev).to(dtype)
+    pos = (torch.arange(B, device=dev) * 31 % (3 * n)).to(torch.int32)
+    mine, ref = both.clone(), both.clone()
+    o = ops.window_attention_step(mine[1, :, 3], mine[0, :, 5], mine[0, :, 7], *mine, pos, H, 64, 5)
+    want = ops.window_attention_step(both[1, :, 3].clone(), both[0, :, 5].clone(), both[0, :, 7].clone(), *ref, pos, H,
+                                     64, 5)
+    assert torch.equal(o, want) and torch.equal(mine, ref)
+    mine, ref = both.clone(), both.clone()
+    ops.window_cache_fill(mine[1].view(B * n, -1), mine[0].view(B * n, -1), n, *mine, 64, 5)
+    ops.window_cache_fill(both[1].view(B * n, -1).clone(), both[0].view(B * n, -1).clone(), n, *ref, 64, 5)
+    assert torch.equal(mine, ref)
+
+
 def test_cache_past_32_bits():
     """A cache of more than 2^31 elements: the last sequence's last slots are read and written."""
     B, KV, D, window = 2, 8, 128, 1_060_000

@@ -23,12 +23,16 @@ def ptr_read(t):
     return fl_ops._pr(t).value
 
 
-def launch(name, args, ints, device):
-    """Calls ``name(&args, *ints, stream)`` on the device's current stream."""
+def launch(name, args, ints, device, refusal=None):
+    """Calls ``name(&args, *ints, stream)`` on the device's current stream. False where it returned ``refusal``, with
+    nothing launched."""
     index = device.index
     if index == torch.cuda.current_device():
         rc = fl_ops._fn(name)(_c.byref(args), *ints, _c.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
     else:
         with torch.cuda.device(device):
             rc = fl_ops._fn(name)(_c.byref(args), *ints, _c.c_void_p(torch._C._cuda_getCurrentRawStream(index)))
+    if rc == refusal:
+        return False
     fl_ops._check(rc, name)
+    return True

@@ -960,6 +960,8 @@ struct StepArgs {
   int start[kMaxBuckets];
 };
 
+constexpr int kRowsInCache = -1;      // what fa_window_step returns, nothing launched, where its rows lie in a cache
+
 // the age (pos − token) of the token in a slot, −1 if there is none; cur = the new token's slot
 __device__ __forceinline__ int slot_age(int s, int pos, int sinks, int W, int cur) {
   if (pos < 0) return -1;
@@ -1255,7 +1257,18 @@ template <typename T, int D> int launch_bwd(const Args& a, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
+// Rows [B][ld], `width` elements of each, that share memory with a cache: the kernel would read them while it writes there
+inline bool rows_in_cache(const StepArgs& a, const void* rows, int64_t ld, int64_t width, int64_t cache, int64_t e) {
+  const char *p = (const char*)rows, *k = (const char*)a.kc, *v = (const char*)a.vc;
+  const int64_t span = ((a.B - 1) * ld + width) * e, size = cache * e;
+  return (p < k + size && p + span > k) || (p < v + size && p + span > v);
+}
+
 template <typename T, int D> int launch_step(const StepArgs& a, hipStream_t st) {
+  const int64_t kv = (int64_t)a.KV * D, cache = (int64_t)a.B * (a.sinks + a.W) * kv, e = sizeof(T);
+  if (rows_in_cache(a, a.q, a.ldq, (int64_t)a.H * D, cache, e) || rows_in_cache(a, a.k, a.ldk, kv, cache, e) ||
+      rows_in_cache(a, a.v, a.ldv, kv, cache, e))
+    return kRowsInCache;
   constexpr int NW = D * sizeof(T) > 256 ? 2 : 4;
   const size_t lds = a.bias ? 32 * a.NB * sizeof(float) + (a.maxd + 4) / 4 * 4 : 0;
   const int64_t n = (int64_t)a.B * a.KV * ((a.H / a.KV + 31) / 32) * a.splits;

@@ -28,6 +28,7 @@ MAX_SINKS = 64
 MAX_BUCKETS = 128
 MAX_DISTANCE = 1024
 _I32 = 2 ** 31 - 1
+_ROWS_IN_CACHE = -1              # fa_window_step launched nothing: its rows lie in a cache that it writes
 
 
 class _Args(_c.Structure):
@@ -333,10 +334,10 @@ def _cache(k_cache, v_cache, B, KV, D, slots, dtype, device):
 
 def _apart(t, caches):
     """The rows, or a copy of rows that lie in a cache, which the call writes while it reads them."""
-    lo = t.data_ptr()
-    hi = lo + ((t.shape[0] - 1) * t.stride(0) + (t.shape[1] - 1) * t.stride(1) + 1) * t.element_size()
+    p = t.data_ptr()
+    span = ((t.shape[0] - 1) * t.stride(0) + (t.shape[1] - 1) * t.stride(1) + 1) * t.element_size()
     k, v, size = caches
-    return t.clone() if (lo < k + size and hi > k) or (lo < v + size and hi > v) else t
+    return t.clone() if -span < p - k < size or -span < p - v < size else t
 
 
 def _pos(pos, B, device, name):
@@ -411,8 +412,8 @@ def window_attention_step(q, k, v, k_cache, v_cache, pos, H: int, window: int, s
         raise ValueError("window_attention_step computes no gradient: call it under torch.no_grad()")
     if B == 0:
         return torch.empty(B, H * D, dtype=q.dtype, device=q.device)
-    q, k, v = _apart(q, caches), _apart(k, caches), _apart(v, caches)
     if not use_native(q):
+        q, k, v = (_apart(t, caches) for t in (q, k, v))
         return _step_ref(q, k, v, k_cache, v_cache, pos, H, KV, W, sinks, table, max_distance, scale)
     o = torch.empty(B, H * D, dtype=q.dtype, device=q.device)
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
@@ -428,7 +429,11 @@ def window_attention_step(q, k, v, k_cache, v_cache, pos, H: int, window: int, s
         part = torch.empty(B * H * a.splits * (D + 2), dtype=torch.float32, device=q.device)
         a.pacc = ptr(part)
         a.pml = a.pacc + 4 * B * H * a.splits * D
-    launch("fa_window_step", a, (q.dtype == torch.bfloat16, D), q.device)
+    if not launch("fa_window_step", a, (q.dtype == torch.bfloat16, D), q.device, _ROWS_IN_CACHE):
+        q, k, v = q.clone(), k.clone(), v.clone()
+        a.q, a.k, a.v = ptr_read(q), ptr_read(k), ptr_read(v)
+        a.ldq, a.ldk, a.ldv = q.stride(0), k.stride(0), v.stride(0)
+        launch("fa_window_step", a, (q.dtype == torch.bfloat16, D), q.device)
     return o
 
 

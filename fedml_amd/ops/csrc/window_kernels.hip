@@ -17,17 +17,19 @@
 //   column operands (products over 32 rows of an LDS tile): the 16 accumulators of a lane ARE the other operand,
 //   with the rows taken in the order κ(r) + 4·hh, so probabilities never leave the registers.
 //
-// Measured on MI355X (a large copy reaches 4.94 TB/s, an 8192³ product 1420 TFLOP/s bf16 and 154 fp32):
-//   forward, bf16:  32768 tokens, 32 heads over 8, D 128, W 1024: 770 us = 714 TFLOP/s; 16 · 1999 (a quarter padding),
-//                   12 heads, D 64, W 256: 98 us
-//   dq / dk, dv:    2 · 16384, 16 heads over 4, D 128, W 1024: 520 / 980 us = 793 / 561 TFLOP/s of the products they
-//                   make (3 and 4 a block); 16 · 1999 as above: 102 / 157 us
-//   step, bf16:     64 caches of 4100 slots, 32 heads over 8, D 128: 225 us = 4.8 TB/s
-// A 32×32 block at D 128 takes the matrix unit 512 cycles forward, 768 in dq and 1024 in dk/dv, the vector unit about
-// 500 in each (16 exponentials a lane at a quarter rate, and what stands around them): the two share the time of a wave,
-// and only other waves of the SIMD fill it — two of them in the forward and dq, one in dk/dv, whose sums, keys and
-// values take 416 registers (keys and values in LDS with two waves a SIMD: 1091 us; two blocks interleaved: spills,
-// 1407 us). At D 64 short windows add the tiles at their edges, which are masked, and a tile's latency at either end.
+// Measured on MI355X (a large copy reaches 4.94 TB/s, an 8192³ product 1420 TFLOP/s bf16 and 154 fp32), medians:
+//   forward, bf16:  32768 tokens, 32 heads over 8, D 128, W 1024: 813 us = 667 TFLOP/s; 16 · 1999 (a quarter padding),
+//                   12 heads, D 64, W 256: 101 us
+//   dq / dk, dv:    2 · 16384, 16 heads over 4, D 128, W 1024: 541 / 994 us = 762 / 553 TFLOP/s of the products they
+//                   make (3 and 4 a block); 16 · 1999 as above: 106 / 157 us
+//   step, bf16:     64 caches of 4100 slots, 32 heads over 8, D 128, with a bias: 239 us = 4.5 TB/s
+// Shares of the wave cycles at these sizes, matrix unit / vector unit / waiting for loads, LDS and barriers / for a turn:
+//   D 128: forward 19 / 26 / 26 / 34 %, dq 20 / 19 / 41 / 28, dk/dv 28 / 25 / 36 / 22;
+//   D 64:  forward 6 / 19 / 37 / 34 %, dq 7 / 15 / 38 / 36, dk/dv 10 / 19 / 45 / 20.
+// The wait is the largest share of both backward passes: a tile is stored to the one LDS buffer, waited for, used and
+// waited for again, with two waves a SIMD in the forward and dq and one in dk/dv at D 128, whose sums, keys and values take
+// 416 registers. At D 64 a short window's walk is 6 or 7 such tiles, half of them at its edges and masked.
+// Tried at D 128: keys and values of dk/dv in LDS with two waves a SIMD 1091 us; two blocks interleaved: spills, 1407 us.
 #include "common.h"
 #include <type_traits>
 
@@ -122,9 +124,9 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
-// A matrix instruction's result may be read 19 instruction slots after its issue (16 passes; 11 for 8). The compiler
-// inserts what is missing, but has been seen to count the longer of two branches between the product and the first use
-// (the last accumulator of 16 was read 11 slots early): wait here, in the product's own block.
+// A product's result may be read 18 instruction slots after its issue at fp32 (16 passes), 12 at bf16 (8). The compiler
+// leaves that much room, but not over every branch: in an earlier form of the biased fp32 forward its assembly read an
+// accumulator 17 slots behind the product. Wait here, in the product's own block, 20 slots for either type.
 __device__ __forceinline__ void settle(f32x16& a) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a)); }
 __device__ __forceinline__ void settle(f32x16& a, f32x16& b) {
   asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a), "+v"(b));
@@ -356,8 +358,9 @@ struct KeyTiles {
 // 256 queries a workgroup are no faster at D 128 and a quarter slower at D 64. At fp32 32 keys keep the registers for
 // two waves a SIMD, and a block's products (4096 cycles at D 64) cover the latency.
 // Probabilities are rounded to the storage type for the product with v (half a step each, 2^-8 in bf16, and the sum is
-// of the unrounded ones). EXACT (bf16, before a gradient of the bias): what that rounding leaves over goes through a
-// second product, so that D = dO·o of the unrounded output is good to 2^-16 — dbias is fp32.
+// of the unrounded ones). EXACT (bf16, before a gradient of the bias): what that rounding leaves over, and what the
+// rounding of this leaves over, go through two more products, so that p in o, and with it D = dO·o of the unrounded
+// output, is good to 2^-24 like the fp32 sums — dbias is fp32.
 // ----------------------------------------------------------------------------------------------------------------
 template <typename T, int D, int NW, int BK, bool BIAS, bool EXACT>
 __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void fwd_kernel(const Args a) {

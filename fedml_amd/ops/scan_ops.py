@@ -3,8 +3,9 @@
     f_t = σ(gate_t),   h_t = f_t·h_{t−1} + (1 − f_t)·x_t,   y_t = h_t
 
 The recurrence is linear in the state, so unlike an LSTM's (:mod:`.rnn_ops`) it needs no product with a weight per step
-and a whole sequence is ONE launch each way. Layout of the recurrent models: ``[C, T, B, H]`` (client, time, sequence,
-feature); any strides with dense features, so token-major rows go in as ``x.view(C, B, T, H).transpose(1, 2)``.
+and a whole sequence is one launch each way, two where few features cut the time into segments. Layout of the recurrent
+models: ``[C, T, B, H]`` (client, time, sequence, feature); any strides with dense features, so token-major rows go in as
+``x.view(C, B, T, H).transpose(1, 2)``.
 
 CUDA tensors run the HIP kernels (bf16 or fp32 storage; states, maps and sums fp32), CPU tensors the same recurrence in
 plain PyTorch (fp64 for fp64 inputs), the tests' oracle. Results are the same bit for bit from call to call. Everything

@@ -12,8 +12,10 @@ Rows are token-major ``[sequences · S, heads · D]``, head h at columns ``[h·D
 (row strides may exceed heads · D: column slices of a fused projection are read in place). CUDA tensors run the HIP
 kernels at the storage precision with fp32 sums and statistics; CPU tensors run the plain-PyTorch form of the same
 mathematics (fp64 for fp64 inputs), which is also the tests' oracle. All results are the same bit for bit from call to
-call: no atomics. Everything is enqueued on the current stream of the tensors' device and may be captured into a HIP
-graph; scratch memory is allocated per call."""
+call: no atomics. (With a bias and bf16 the output's bits differ between calls with and without a gradient of the bias:
+before one, the probabilities go into it unrounded.) Everything is enqueued on the current stream of the tensors' device
+and may be captured into a HIP graph, forward and backward in the same one, on leaves that no living eager graph holds;
+scratch memory is allocated per call."""
 import ctypes as _c
 import functools
 import math
@@ -188,16 +190,23 @@ def _plan(D, N, S, H, KV, W, sinks, scale, fp32, C, buckets, max_distance, train
         a.start[:buckets] = relative_bucket_starts(buckets, max_distance)
     # Queries of a workgroup, forward and dq: one wave's 32 for short sequences, and at fp32, where products are 16 times
     # as long, wherever no more than 1024 such waves are there (a wave then walks its own keys, not its workgroup's).
-    # us forward + backward, 128 / 32 queries: fp32 [80·80, 4 heads] 19 + 73 / 15 + 72, [16·256, 4] 23 + 81 / 17 + 72,
-    # [64·128, 12] 37 + 152 / 45 + 163; bf16 [16·256, 4] 10 + 31 / 8 + 30, [2·2048, 8] 19 + 59 / 23 + 71.
+    # us forward + backward, 128 / 32 queries, at windows of 32, 128 and 512:
+    #   fp32 [80·80, 4 heads] 81 / 67, 86 / 80; [16·256, 4] 61 / 44, 94 / 78, 102 / 107; [2·1000, 8] 63 / 45, 96 / 80,
+    #   220 / 215; [4·256, 8, D 128] 123 / 88, 183 / 151, 185 / 188; more waves: [64·128, 12] W 32 152 / 138, W 512
+    #   173 / 192; [8·1024, 8] W 32 118 / 99, W 512 413 / 416;
+    #   bf16 [64·20, 4] 15 / 15; [16·256, 4] 28 / 24, 33 / 32, 33 / 38; [2·2048, 8] 32 / 30, 38 / 39, 62 / 72.
+    # Windows up to 64 gain from 32 queries on the other side of the rule too; the rule does not look at them.
     a.tile = 32 if S <= 64 or (fp32 and N * H * -(-S // 32) <= 1024) else 128
-    # Keys of a workgroup, dk and dv: 64 for short sequences and at fp32 (forward + backward, 128 / 64 keys, W 512:
-    # [8·2048, 8 heads] 977 / 898 us, [2·2048, 8] 336 / 280; bf16 189 / 190), but 128 at fp32 and 128 dims, where two
-    # waves would spill (1874 / 1951).
+    # Keys of a workgroup, dk and dv: 64 for short sequences and at fp32, but 128 at fp32 and 128 dims, where two waves
+    # would spill. us forward + backward, 128 / 64 keys, W 512: fp32 [8·2048, 8 heads] 862 / 829, [2·2048, 8] 239 / 237,
+    # [16·256, 4] 108 / 106; bf16 [8·2048, 8] 162 / 162, [2·2048, 8] 64 / 69, [16·256, 4] 33 / 33, [4·4096, 8 over 2,
+    # D 128, W 1024] 426 / 495.
     a.ktile = 64 if (S <= 64 or fp32) and not (fp32 and D == 128) else 128
     # The sinks' gradients from behind their window: up to 512 queries are walked by the sinks' own keys, more by a pass
-    # of its own in chunks about as long as a window's walk ([80·80, 4 heads] fp32, 48 such queries: dk/dv 54 us with
-    # the pass, 45 without).
+    # of its own in chunks about as long as a window's walk. us forward + backward with the pass / without, for 128, 256,
+    # 512 and 1024 such queries: bf16 [2 sequences, 8 heads, W 64] 29 / 27, 33 / 36, 36 / 44, 38 / 62; [16, 12 heads,
+    # W 256] 79 / 74, 97 / 102, 139 / 150, 219 / 245; [2, 16 over 4, D 128, W 256] 113 / 114, 118 / 142, 121 / 193,
+    # 138 / 302; fp32 [16, 12 heads, W 256] 293 / 290, 417 / 471, 618 / 727, 1013 / 1273. It pays from 256 queries on.
     if sinks and S - W > 512:
         a.qchunk = max(512, -(-(W + 128) // 128) * 128)
         a.nchunk = -(-(S - W) // a.qchunk)
